@@ -110,6 +110,32 @@ SIGNATURES = {
     "cta_causal_self_attention_bwd_workspace": (_i64, [_i64, _i64]),
     "cta_causal_self_attention_bwd": (_int, [_p, _i64p, _p, _i64p, _p, _i64p, _p, _p, _i64p,
                                              _i64, _i64, _i64, _p, _p, _p, _p, _p]),
+    "cta_paged_kv_append": (_int, [_p, _i64p, _p, _i64p, _p, _i64p, _i64, _i64, _i64, _i64, _p, _p,
+                                 _i64, _int, _p, _i64p, _p, _i64p, _i64, _i64, _p, _i64, _i64, _p,
+                                 _p, _i64, _p, _p]),
+    "cta_paged_attention_decode": (_int, [_p, _i64p, _p, _i64p, _p, _i64p, _i64, _i64, _p, _i64, _i64,
+                                        _p, _i64, _i64, _i64, _i64, _f32, _p, _p, _p, _i64, _p]),
+    "cta_paged_attention_prefill": (_int, [_p, _i64p, _p, _i64p, _p, _i64p, _i64, _i64, _p, _i64,
+                                         _i64, _p, _p, _i64, _i64, _i64, _i64, _i64, _f32, _p, _p,
+                                         _p, _i64, _p]),
+    "cta_paged_kv_append_bf16": (_int, [_p, _i64p, _p, _i64p, _p, _i64p, _i64, _i64, _i64, _i64, _p, _p,
+                                 _i64, _int, _p, _i64p, _p, _i64p, _i64, _i64, _p, _i64, _i64, _p,
+                                 _p, _i64, _p, _p]),
+    "cta_paged_attention_decode_bf16": (_int, [_p, _i64p, _p, _i64p, _p, _i64p, _i64, _i64, _p, _i64, _i64,
+                                        _p, _i64, _i64, _i64, _i64, _f32, _p, _p, _p, _i64, _p]),
+    "cta_paged_attention_prefill_bf16": (_int, [_p, _i64p, _p, _i64p, _p, _i64p, _i64, _i64, _p, _i64,
+                                         _i64, _p, _p, _i64, _i64, _i64, _i64, _i64, _f32, _p, _p,
+                                         _p, _i64, _p]),
+    "cta_paged_kv_append_f16": (_int, [_p, _i64p, _p, _i64p, _p, _i64p, _i64, _i64, _i64, _i64, _p, _p,
+                                 _i64, _int, _p, _i64p, _p, _i64p, _i64, _i64, _p, _i64, _i64, _p,
+                                 _p, _i64, _p, _p]),
+    "cta_paged_attention_decode_f16": (_int, [_p, _i64p, _p, _i64p, _p, _i64p, _i64, _i64, _p, _i64, _i64,
+                                        _p, _i64, _i64, _i64, _i64, _f32, _p, _p, _p, _i64, _p]),
+    "cta_paged_attention_prefill_f16": (_int, [_p, _i64p, _p, _i64p, _p, _i64p, _i64, _i64, _p, _i64,
+                                         _i64, _p, _p, _i64, _i64, _i64, _i64, _i64, _f32, _p, _p,
+                                         _p, _i64, _p]),
+    "cta_paged_attention_decode_workspace": (_i64, [_i64] * 6),
+    "cta_paged_attention_prefill_workspace": (_i64, [_i64] * 7),
 }
 
 

@@ -5,8 +5,8 @@
 // validates its inputs with TORCH_CHECK (surfacing as a Python RuntimeError), allocates
 // dense outputs on the input's device, and calls the gfx950 kernels through the C ABI on
 // torch's current HIP stream.  Two schemas are added for LayerNorm, which the reference
-// implements in plain torch only (gpt/gpt.py:47-59), and two for the fused linear+GELU products
-// of the GPT MLP.
+// implements in plain torch only (gpt/gpt.py:47-59), two for the fused linear+GELU products
+// of the GPT MLP, and those of the paged key/value cache.
 //
 // This file is host-only C++; every kernel lives in libcuda_transformer_amd.so.
 #include <Python.h>
@@ -19,6 +19,7 @@
 #include <algorithm>
 #include <array>
 #include <atomic>
+#include <cmath>
 #include <cstdint>
 #include <tuple>
 
@@ -845,6 +846,250 @@ at::Tensor flash_attention_qkv_bwd(at::Tensor qkv, at::Tensor out, at::Tensor do
   return dqkv;
 }
 
+// ------------------------------------------------------------------ paged key/value cache
+// New ops with no reference counterpart: a cache of keys and values in pages, what is appended to
+// it and the attention of new tokens over it (include/cuda_transformer_amd.h says what the plan
+// tensors hold).  The plan stays on the device: nothing here waits for it.
+
+// The caches are read and written where they are, so a layout that the kernels cannot take is an
+// error here, not a copy.
+void check_cache(const at::Tensor& c, const char* name, const at::Tensor& x) {
+  TORCH_CHECK(c.dim() == 4, name, " must be a 4D tensor (pages, kv heads, page size, hs)");
+  TORCH_CHECK(c.is_cuda() && c.device() == x.device(), name, " must be on the device of ",
+              "the other tensors");
+  TORCH_CHECK(c.scalar_type() == x.scalar_type(), name, " must have the dtype of the tokens (",
+              x.scalar_type(), "), got ", c.scalar_type());
+  const int64_t vec = 16 / c.element_size();
+  const auto s = strides_of<4>(c);
+  TORCH_CHECK((c.size(3) == 1 || c.stride(3) == 1) && s[0] % vec == 0 && s[1] % vec == 0 &&
+                  s[2] % vec == 0 && (reinterpret_cast<uintptr_t>(c.data_ptr()) & 15u) == 0,
+              name, " needs a unit last stride and 16-byte aligned rows");
+}
+
+struct PagedPlanTensors {
+  at::Tensor table, lens, cu;
+  int64_t table_stride, pages_per_seq, B;
+  const int32_t* cu_ptr() const { return cu.defined() ? cu.data_ptr<int32_t>() : nullptr; }
+};
+
+PagedPlanTensors check_plan(const at::Tensor& page_table, const at::Tensor& seq_lens,
+                            const c10::optional<at::Tensor>& cu_q, const at::Tensor& x) {
+  TORCH_CHECK(page_table.dim() == 2, "page_table must be a 2D tensor (sequences, pages)");
+  TORCH_CHECK(seq_lens.dim() == 1 && seq_lens.size(0) == page_table.size(0),
+              "seq_lens must have one entry per row of page_table");
+  PagedPlanTensors p;
+  p.B = page_table.size(0);
+  p.pages_per_seq = page_table.size(1);
+  auto check = [&](const at::Tensor& t, const char* name) {
+    TORCH_CHECK(t.is_cuda() && t.device() == x.device(), name, " must be on the device of ",
+                "the other tensors");
+    TORCH_CHECK(t.scalar_type() == at::kInt, name, " must be an int32 tensor, got ",
+                t.scalar_type());
+  };
+  check(page_table, "page_table");
+  check(seq_lens, "seq_lens");
+  p.table = p.pages_per_seq == 0 || page_table.stride(1) == 1 ? page_table : page_table.contiguous();
+  p.table_stride = p.table.stride(0);
+  p.lens = seq_lens.contiguous();
+  if (cu_q) {
+    check(*cu_q, "cu_q");
+    TORCH_CHECK(cu_q->dim() == 1 && cu_q->size(0) == p.B + 1,
+                "cu_q must have one entry more than seq_lens");
+    p.cu = cu_q->contiguous();
+  }
+  return p;
+}
+
+// Packed tokens (N, heads, hs) as the kernels read them: dense heads in 16-byte rows, or a copy.
+at::Tensor tokens_operand(const at::Tensor& t) {
+  const int64_t vec = 16 / t.element_size();
+  const auto s = strides_of<3>(t);
+  const bool ok = (t.size(2) == 1 || t.stride(2) == 1) && s[0] % vec == 0 && s[1] % vec == 0 &&
+                  (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15u) == 0;
+  return ok ? t : dense(t);
+}
+
+void check_serving_dtype(const at::Tensor& t, const char* name) {
+  TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor");
+  TORCH_CHECK(t.scalar_type() == at::kFloat || is_half16(t), name,
+              " must be a float32, bfloat16 or float16 tensor, got ", t.scalar_type());
+}
+
+// q (N, nh, hs) or none, k and v (N, nkv, hs).  Returns the rotated q.
+at::Tensor paged_append_impl(const c10::optional<at::Tensor>& q, const at::Tensor& k,
+                             const at::Tensor& v, const c10::optional<at::Tensor>& cos,
+                             const c10::optional<at::Tensor>& sin, bool interleaved,
+                             const at::Tensor& k_cache, const at::Tensor& v_cache,
+                             const at::Tensor& page_table, const at::Tensor& seq_lens,
+                             const c10::optional<at::Tensor>& cu_q) {
+  TORCH_CHECK(k.dim() == 3, "k must be a 3D tensor (tokens, kv heads, hs)");
+  check_serving_dtype(k, "k");
+  TORCH_CHECK(v.sizes() == k.sizes() && v.scalar_type() == k.scalar_type() &&
+                  v.device() == k.device(),
+              "k and v must have the same shape, dtype and device");
+  const int64_t N = k.size(0), nkv = k.size(1), hs = k.size(2);
+  TORCH_CHECK(hs == 32 || hs == 64 || hs == 128,
+              "Unsupported head dimension! Only hs=32, hs=64, and hs=128 are supported.");
+  check_cache(k_cache, "k_cache", k);
+  check_cache(v_cache, "v_cache", k);
+  TORCH_CHECK(k_cache.sizes() == v_cache.sizes(), "k_cache and v_cache must have the same shape");
+  TORCH_CHECK(k_cache.size(1) == nkv && k_cache.size(3) == hs,
+              "the caches must have the kv heads and head size of k");
+  for (const auto* c : {&k_cache, &v_cache})
+    for (int64_t d = 0; d < 3; ++d)
+      TORCH_CHECK(c->size(d) <= 1 || c->stride(d) > 0,
+                  "the caches are written in place and cannot be expanded tensors");
+  const PagedPlanTensors p = check_plan(page_table, seq_lens, cu_q, k);
+  if (!cu_q) TORCH_CHECK(N == p.B, "without cu_q there must be one token per sequence");
+  int64_t nh = 0, rot = 0;
+  at::Tensor qd, cd, sd, q_out;
+  if (q) {
+    TORCH_CHECK(q->dim() == 3 && q->size(0) == N && q->size(2) == hs,
+                "q must be a 3D tensor (tokens, heads, hs) with the tokens and head size of k");
+    TORCH_CHECK(q->scalar_type() == k.scalar_type() && q->device() == k.device(),
+                "q must have the dtype and device of k");
+    nh = q->size(1);
+    TORCH_CHECK(nkv > 0 && nh % nkv == 0, "q must have a multiple of the kv heads");
+    TORCH_CHECK(cos->dim() == 2 && cos->sizes() == sin->sizes(),
+                "cos and sin must be 2D tensors (positions, rotated size / 2) of one shape");
+    for (const auto* t : {&*cos, &*sin})
+      TORCH_CHECK(t->is_cuda() && t->device() == k.device() && t->scalar_type() == at::kFloat,
+                  "cos and sin must be float32 tensors on the device of k");
+    rot = 2 * cos->size(1);
+    TORCH_CHECK(rot % 16 == 0 && rot > 0 && rot <= hs,
+                "the rotated size, 2 * cos.size(1), must be a multiple of 16 up to the head size");
+    TORCH_CHECK(cos->size(0) >= p.pages_per_seq * k_cache.size(2),
+                "cos and sin must cover every position of page_table (", p.pages_per_seq, " pages of ",
+                k_cache.size(2), ")");
+  }
+  c10::OptionalDeviceGuard guard(k.device());
+  if (q) {
+    qd = tokens_operand(*q);
+    cd = dense(*cos);
+    sd = dense(*sin);
+    q_out = at::empty({N, nh, hs}, k.options());
+  }
+  const at::Tensor kd = tokens_operand(k), vd = tokens_operand(v);
+  const auto ks = strides_of<3>(kd), vs = strides_of<3>(vd);
+  const auto qs = q ? strides_of<3>(qd) : ks;
+  const int64_t unit_q[3] = {qs[0], qs[1], 1}, unit_k[3] = {ks[0], ks[1], 1},
+                unit_v[3] = {vs[0], vs[1], 1};
+  const auto kc = strides_of<4>(k_cache), vc = strides_of<4>(v_cache);
+  const int64_t kcs[4] = {kc[0], kc[1], kc[2], 1}, vcs[4] = {vc[0], vc[1], vc[2], 1};
+  auto call = [&]<class P>(auto fn, P*) {
+    check_rc(fn(q ? static_cast<const P*>(qd.data_ptr()) : nullptr, unit_q,
+                static_cast<const P*>(kd.data_ptr()), unit_k,
+                static_cast<const P*>(vd.data_ptr()), unit_v, N, nh, nkv, hs,
+                q ? cd.data_ptr<float>() : nullptr, q ? sd.data_ptr<float>() : nullptr, rot,
+                interleaved ? 1 : 0, static_cast<P*>(k_cache.data_ptr()), kcs,
+                static_cast<P*>(v_cache.data_ptr()), vcs, k_cache.size(0), k_cache.size(2),
+                p.table.data_ptr<int32_t>(), p.table_stride, p.pages_per_seq,
+                p.lens.data_ptr<int32_t>(), p.cu_ptr(), p.B,
+                q ? static_cast<P*>(q_out.data_ptr()) : nullptr, stream_of(k)));
+  };
+  if (k.scalar_type() == at::kFloat) call(cta_paged_kv_append, static_cast<float*>(nullptr));
+  else call(k.scalar_type() == at::kBFloat16 ? cta_paged_kv_append_bf16 : cta_paged_kv_append_f16,
+            static_cast<uint16_t*>(nullptr));
+  return q_out;
+}
+
+void paged_kv_append(at::Tensor k, at::Tensor v, at::Tensor k_cache, at::Tensor v_cache,
+                     at::Tensor page_table, at::Tensor seq_lens, c10::optional<at::Tensor> cu_q) {
+  paged_append_impl(c10::nullopt, k, v, c10::nullopt, c10::nullopt, false, k_cache, v_cache,
+                    page_table, seq_lens, cu_q);
+}
+
+at::Tensor paged_kv_append_rotary(at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor cos,
+                                  at::Tensor sin, at::Tensor k_cache, at::Tensor v_cache,
+                                  at::Tensor page_table, at::Tensor seq_lens,
+                                  c10::optional<at::Tensor> cu_q, bool interleaved) {
+  return paged_append_impl(q, k, v, cos, sin, interleaved, k_cache, v_cache, page_table, seq_lens,
+                           cu_q);
+}
+
+// Attention of q (rows, nh, hs); without cu_q one row a sequence.
+std::tuple<at::Tensor, at::Tensor> paged_attention_impl(
+    const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache,
+    const at::Tensor& page_table, const at::Tensor& seq_lens,
+    const c10::optional<at::Tensor>& cu_q, c10::optional<double> scale) {
+  TORCH_CHECK(q.dim() == 3, "q must be a 3D tensor (tokens, heads, hs)");
+  check_serving_dtype(q, "q");
+  const int64_t rows = q.size(0), nh = q.size(1), hs = q.size(2);
+  TORCH_CHECK(hs == 32 || hs == 64 || hs == 128,
+              "Unsupported head dimension! Only hs=32, hs=64, and hs=128 are supported.");
+  check_cache(k_cache, "k_cache", q);
+  check_cache(v_cache, "v_cache", q);
+  TORCH_CHECK(k_cache.sizes() == v_cache.sizes(), "k_cache and v_cache must have the same shape");
+  const int64_t nkv = k_cache.size(1);
+  TORCH_CHECK(nkv > 0 && nh % nkv == 0, "q must have a multiple of the kv heads");
+  TORCH_CHECK(k_cache.size(3) == hs, "the caches must have the head size of q");
+  const PagedPlanTensors p = check_plan(page_table, seq_lens, cu_q, q);
+  if (!cu_q) TORCH_CHECK(rows == p.B, "q must have one token per sequence");
+  const double sc = scale ? *scale : 1.0 / std::sqrt(static_cast<double>(hs));
+  TORCH_CHECK(std::isfinite(static_cast<float>(sc)), "scale must be finite");
+  c10::OptionalDeviceGuard guard(q.device());
+  at::Tensor O = at::empty({rows, nh, hs}, q.options());
+  at::Tensor L = at::empty({rows, nh}, q.options().dtype(at::kFloat));
+  const at::Tensor qd = tokens_operand(q);
+  const auto qs = strides_of<3>(qd);
+  const int64_t unit_q[3] = {qs[0], qs[1], 1};
+  const auto kc = strides_of<4>(k_cache), vc = strides_of<4>(v_cache);
+  const int64_t kcs[4] = {kc[0], kc[1], kc[2], 1}, vcs[4] = {vc[0], vc[1], vc[2], 1};
+  const int64_t pages = k_cache.size(0), ps = k_cache.size(2);
+  TORCH_CHECK(ps > 0, "page_size must be at least 1");
+  const int64_t ws_bytes =
+      cu_q ? cta_paged_attention_prefill_workspace(p.B, rows, nh, nkv, hs, p.pages_per_seq, ps)
+           : cta_paged_attention_decode_workspace(p.B, nh, nkv, hs, p.pages_per_seq, ps);
+  at::Tensor ws;
+  if (ws_bytes > 0) ws = at::empty({(ws_bytes + 3) / 4}, q.options().dtype(at::kFloat));
+  void* wp = ws_bytes > 0 ? ws.data_ptr() : nullptr;
+  auto decode = [&]<class P>(auto fn, P*) {
+    check_rc(fn(static_cast<const P*>(qd.data_ptr()), unit_q,
+                static_cast<const P*>(k_cache.data_ptr()), kcs,
+                static_cast<const P*>(v_cache.data_ptr()), vcs, pages, ps,
+                p.table.data_ptr<int32_t>(), p.table_stride, p.pages_per_seq,
+                p.lens.data_ptr<int32_t>(), p.B, nh, nkv, hs, static_cast<float>(sc),
+                static_cast<P*>(O.data_ptr()), L.data_ptr<float>(), wp, ws_bytes, stream_of(q)));
+  };
+  auto prefill = [&]<class P>(auto fn, P*) {
+    check_rc(fn(static_cast<const P*>(qd.data_ptr()), unit_q,
+                static_cast<const P*>(k_cache.data_ptr()), kcs,
+                static_cast<const P*>(v_cache.data_ptr()), vcs, pages, ps,
+                p.table.data_ptr<int32_t>(), p.table_stride, p.pages_per_seq,
+                p.lens.data_ptr<int32_t>(), p.cu_ptr(), p.B, rows, nh, nkv, hs,
+                static_cast<float>(sc), static_cast<P*>(O.data_ptr()), L.data_ptr<float>(), wp,
+                ws_bytes, stream_of(q)));
+  };
+  float* const f32 = nullptr;
+  uint16_t* const u16 = nullptr;
+  const bool bf = q.scalar_type() == at::kBFloat16;
+  if (q.scalar_type() == at::kFloat) {
+    if (cu_q) prefill(cta_paged_attention_prefill, f32);
+    else decode(cta_paged_attention_decode, f32);
+  } else if (cu_q) {
+    prefill(bf ? cta_paged_attention_prefill_bf16 : cta_paged_attention_prefill_f16, u16);
+  } else {
+    decode(bf ? cta_paged_attention_decode_bf16 : cta_paged_attention_decode_f16, u16);
+  }
+  return {O, L};
+}
+
+std::tuple<at::Tensor, at::Tensor> paged_attention_decode(at::Tensor q, at::Tensor k_cache,
+                                                          at::Tensor v_cache,
+                                                          at::Tensor page_table,
+                                                          at::Tensor seq_lens,
+                                                          c10::optional<double> scale) {
+  return paged_attention_impl(q, k_cache, v_cache, page_table, seq_lens, c10::nullopt, scale);
+}
+
+std::tuple<at::Tensor, at::Tensor> paged_attention_prefill(at::Tensor q, at::Tensor k_cache,
+                                                           at::Tensor v_cache,
+                                                           at::Tensor page_table,
+                                                           at::Tensor seq_lens, at::Tensor cu_q,
+                                                           c10::optional<double> scale) {
+  return paged_attention_impl(q, k_cache, v_cache, page_table, seq_lens, cu_q, scale);
+}
+
 }  // namespace
 
 TORCH_LIBRARY(cuda_transformer, m) {
@@ -884,6 +1129,19 @@ TORCH_LIBRARY(cuda_transformer, m) {
   m.def(
       "layernorm_bwd(Tensor x, Tensor gamma, Tensor mean, Tensor rstd, Tensor dy) -> "
       "(Tensor, Tensor, Tensor)");
+  m.def(
+      "paged_kv_append(Tensor k, Tensor v, Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor "
+      "page_table, Tensor seq_lens, Tensor? cu_q) -> ()");
+  m.def(
+      "paged_kv_append_rotary(Tensor q, Tensor k, Tensor v, Tensor cos, Tensor sin, Tensor(a!) "
+      "k_cache, Tensor(b!) v_cache, Tensor page_table, Tensor seq_lens, Tensor? cu_q, bool "
+      "interleaved) -> Tensor");
+  m.def(
+      "paged_attention_decode(Tensor q, Tensor k_cache, Tensor v_cache, Tensor page_table, Tensor "
+      "seq_lens, float? scale) -> (Tensor, Tensor)");
+  m.def(
+      "paged_attention_prefill(Tensor q, Tensor k_cache, Tensor v_cache, Tensor page_table, Tensor "
+      "seq_lens, Tensor cu_q, float? scale) -> (Tensor, Tensor)");
 }
 
 TORCH_LIBRARY_IMPL(cuda_transformer, CUDA, m) {
@@ -913,6 +1171,10 @@ TORCH_LIBRARY_IMPL(cuda_transformer, CUDA, m) {
   m.impl("layernorm_bwd", &layernorm_bwd);
   m.impl("add_layernorm_fwd", &add_layernorm_fwd);
   m.impl("add_layernorm_bwd", &add_layernorm_bwd);
+  m.impl("paged_kv_append", &paged_kv_append);
+  m.impl("paged_kv_append_rotary", &paged_kv_append_rotary);
+  m.impl("paged_attention_decode", &paged_attention_decode);
+  m.impl("paged_attention_prefill", &paged_attention_prefill);
 }
 
 }  // namespace cuda_transformer

@@ -13,8 +13,12 @@ Added: ``layernorm_fwd`` / ``layernorm_bwd`` (the reference's LayerNorm is plain
 gpt/gpt.py:47-59), and ``cuda_fma_gelu`` / ``cuda_fma_gelu_grad``, the GPT MLP's linear+GELU
 pairs (gpt/gpt.py:134-135 and their backward) fused into one GEMM each, and
 ``gelu_tanh_activation`` / ``gelu_tanh_activation_bwd``, the tanh-approximated GELU (with its
-fused linear pair ``cuda_fma_gelu_tanh`` / ``cuda_fma_gelu_tanh_grad``).
+fused linear pair ``cuda_fma_gelu_tanh`` / ``cuda_fma_gelu_tanh_grad``), and the serving
+operators on a paged key/value cache, ``paged_kv_append``, ``paged_attention_decode`` and
+``paged_attention_prefill``.
 """
+from typing import Optional
+
 import torch
 from torch import Tensor
 
@@ -27,6 +31,7 @@ __all__ = [
     "flash_attention_fwd", "flash_attention_bwd",
     "flash_attention_qkv_fwd", "flash_attention_qkv_bwd",
     "layernorm_fwd", "layernorm_bwd", "add_layernorm_fwd", "add_layernorm_bwd",
+    "paged_kv_append", "paged_attention_decode", "paged_attention_prefill",
 ]
 
 _ops = torch.ops.cuda_transformer
@@ -418,3 +423,99 @@ def _(xsum, gamma, mean, rstd, dy, dres):
     n = xsum.size(-1)
     return (torch.empty_like(xsum), torch.empty(n, dtype=xsum.dtype, device=xsum.device),
             torch.empty(n, dtype=xsum.dtype, device=xsum.device))
+
+
+# ----------------------------------------------------------------- paged key/value cache (added)
+# Shared by the three operators.  k_cache and v_cache are pools of pages, (pages, kv heads, page
+# size, hs), of any page size, read and written in place: unit last stride, 16-byte aligned rows (a
+# transposed view of a (pages, page size, kv heads, hs) pool is fine).  The plan is int32 tensors on
+# the device, which no call waits for:
+#   page_table (B, P): sequence b's pages in order.  An entry outside [0, pages) maps no page: its
+#       positions hold no key, and nothing is stored there.
+#   seq_lens (B,): each sequence's length with its new tokens; 0 for an empty slot of the batch.
+#   cu_q (B + 1,): packed rows cu_q[b] .. cu_q[b + 1] - 1 are the new tokens of sequence b, its last
+#       positions.  Rows behind cu_q[B] are padding.
+# Sequences may share pages that none of them appends to.  The caches have no gradient.
+def paged_kv_append(k: Tensor, v: Tensor, k_cache: Tensor, v_cache: Tensor, page_table: Tensor,
+                    seq_lens: Tensor, cu_q: Optional[Tensor] = None, q: Optional[Tensor] = None,
+                    cos: Optional[Tensor] = None, sin: Optional[Tensor] = None,
+                    interleaved: bool = False) -> Optional[Tensor]:
+    """Store the keys and values of new tokens, k and v (N, kv heads, hs), in the paged cache.
+
+    Without cu_q there is one new token a sequence (N = B).  Tokens outside their sequence's pages
+    are not stored.  With q (N, heads, hs), cos and sin (positions, rot / 2; float32, a row for every
+    position of page_table), q and k are rotated by their positions first and the rotated q is
+    returned: of the first ``rot`` elements (a multiple of 16) the pairs (x, y) of elements i and
+    i + rot / 2 (2i and 2i + 1 if ``interleaved``) become (x cos - y sin, y cos + x sin), in FP32,
+    rounded once.  q of a token without a position (padding) comes back as it is."""
+    if q is None:
+        torch._check(cos is None and sin is None, lambda: "cos and sin are taken together with q")
+        _ops.paged_kv_append.default(k, v, k_cache, v_cache, page_table, seq_lens, cu_q)
+        return None
+    torch._check(cos is not None and sin is not None, lambda: "q is taken together with cos and sin")
+    return _ops.paged_kv_append_rotary.default(q, k, v, cos, sin, k_cache, v_cache, page_table,
+                                               seq_lens, cu_q, interleaved)
+
+
+def _check_paged(x, k_cache, v_cache, page_table, seq_lens, cu_q=None):
+    torch._check(x.dtype in (torch.float32, torch.bfloat16, torch.float16))
+    torch._check(k_cache.dtype == x.dtype and v_cache.dtype == x.dtype,
+                 lambda: "the caches must have the dtype of the tokens")
+    torch._check(x.dim() == 3 and k_cache.dim() == 4 and k_cache.shape == v_cache.shape)
+    torch._check(x.size(2) == k_cache.size(3), lambda: "the caches must have the tokens' head size")
+    torch._check(page_table.dim() == 2 and seq_lens.dim() == 1
+                 and seq_lens.size(0) == page_table.size(0))
+    plan = (page_table, seq_lens) if cu_q is None else (page_table, seq_lens, cu_q)
+    for t in plan:
+        torch._check(t.dtype == torch.int32, lambda: "the plan tensors must be int32")
+    _same_device(x, k_cache, v_cache, *plan)
+
+
+@torch.library.register_fake("cuda_transformer::paged_kv_append")
+def _(k, v, k_cache, v_cache, page_table, seq_lens, cu_q):
+    _check_paged(k, k_cache, v_cache, page_table, seq_lens, cu_q)
+    torch._check(v.shape == k.shape and v.dtype == k.dtype)
+
+
+@torch.library.register_fake("cuda_transformer::paged_kv_append_rotary")
+def _(q, k, v, cos, sin, k_cache, v_cache, page_table, seq_lens, cu_q, interleaved):
+    _check_paged(k, k_cache, v_cache, page_table, seq_lens, cu_q)
+    torch._check(v.shape == k.shape and v.dtype == k.dtype and q.dtype == k.dtype)
+    _f32(cos, sin)
+    return torch.empty(q.shape, dtype=q.dtype, device=q.device)
+
+
+def paged_attention_decode(q: Tensor, k_cache: Tensor, v_cache: Tensor, page_table: Tensor,
+                           seq_lens: Tensor, scale: Optional[float] = None) -> tuple[Tensor, Tensor]:
+    """Attention of one new token a sequence, q (B, heads, hs), over its cached positions 0 ..
+    seq_lens[b] - 1 (its own is appended first) -> (O (B, heads, hs), L (B, heads)).
+
+    ``heads`` is a multiple of the cache's kv heads; query head h reads kv head h // (heads // kv
+    heads).  Scores are scale q.k, scale = 1/sqrt(hs) unless given; L = rowmax + ln(rowsum) in
+    float32.  A row without a key gives O = 0 and L = -inf."""
+    return _ops.paged_attention_decode.default(q, k_cache, v_cache, page_table, seq_lens, scale)
+
+
+@torch.library.register_fake("cuda_transformer::paged_attention_decode")
+def _(q, k_cache, v_cache, page_table, seq_lens, scale):
+    _check_paged(q, k_cache, v_cache, page_table, seq_lens)
+    return (torch.empty(q.shape, dtype=q.dtype, device=q.device),
+            torch.empty(q.shape[:2], dtype=torch.float32, device=q.device))
+
+
+def paged_attention_prefill(q: Tensor, k_cache: Tensor, v_cache: Tensor, page_table: Tensor,
+                            seq_lens: Tensor, cu_q: Tensor,
+                            scale: Optional[float] = None) -> tuple[Tensor, Tensor]:
+    """Attention of packed new tokens, q (N, heads, hs), over the cache that already holds them ->
+    (O (N, heads, hs), L (N, heads)): prompts, chunks of prompts behind a cached context, drafts.
+    Each token sees its sequence's positions up to its own.  Heads, scale and L as in
+    ``paged_attention_decode``; padding rows give O = 0 and L = -inf."""
+    return _ops.paged_attention_prefill.default(q, k_cache, v_cache, page_table, seq_lens, cu_q,
+                                                scale)
+
+
+@torch.library.register_fake("cuda_transformer::paged_attention_prefill")
+def _(q, k_cache, v_cache, page_table, seq_lens, cu_q, scale):
+    _check_paged(q, k_cache, v_cache, page_table, seq_lens, cu_q)
+    return (torch.empty(q.shape, dtype=q.dtype, device=q.device),
+            torch.empty(q.shape[:2], dtype=torch.float32, device=q.device))

@@ -8,7 +8,7 @@
  * on top of these functions.
  *
  * Conventions shared by every entry point
- *  - Tensors are FP32, device-resident (HIP device pointers).
+ *  - Tensors are FP32 unless an entry says otherwise, device-resident (HIP device pointers).
  *  - Strides are in elements, outermost first.  Outputs are always dense
  *    row-major ("contiguous"), exactly as the reference launchers allocate them.
  *  - `stream` is a hipStream_t passed as void* (NULL = the null stream).  Every
@@ -514,6 +514,116 @@ int cta_causal_self_attention_bwd(const float* q, const int64_t* q_strides,
                                   int64_t BH, int64_t T, int64_t hs,
                                   float* dq, float* dk, float* dv, float* workspace,
                                   void* stream);
+
+/* ------------------------------------------------------------------------------
+ * Serving: a paged key/value cache, what is appended to it and the attention over it.  No
+ * reference counterpart.  FP32, and BF16 / FP16 (raw 16-bit patterns) with the suffix.
+ *
+ * The caches are pools of pages, (num_pages, nkv, page_size, hs), strides (page, head, row, d):
+ * unit d-stride, the others non-negative multiples of 16 bytes, 16-byte aligned bases.  Any
+ * page_size.  page_table row b (pages_per_seq entries, rows table_stride apart) lists sequence b's
+ * pages in order: position p is row p % page_size of page page_table[b][p / page_size].
+ * seq_lens[b] counts sequence b's tokens, new ones included.  New tokens are packed: rows
+ * cu_q[b] .. cu_q[b+1] - 1 (cu_q: B + 1 entries) are the last ones of sequence b.  Packed tensors
+ * (token, head, d) have strides of 3 entries, unit d-stride, rows 16-byte aligned.
+ *
+ * page_table, seq_lens and cu_q are device memory and are not looked at by the host; no value in
+ * them makes a kernel read or write outside the buffers.  An entry of the table outside
+ * [0, num_pages) maps no page, and positions outside [0, pages_per_seq * page_size) (at most 2^30)
+ * have none: they hold no key, and nothing is stored there.  Packed rows that belong to no
+ * sequence (behind cu_q[B]) are padding.  Sequences may share pages that none of them appends to.
+ * ---------------------------------------------------------------------------- */
+
+/* Stores k and v (N, nkv, hs) at their tokens' positions.  rot > 0 (a multiple of 16 up to hs):
+ * k, and q (N, nh, hs) into q_out (dense), are rotated by their positions: pairs (x, y) of elements
+ * i and i + rot/2, or 2i and 2i + 1 if interleaved, become (x c - y s, y c + x s) with
+ * c = cos[pos][i], s = sin[pos][i]; cos and sin dense FP32 (pages_per_seq * page_size, rot/2),
+ * 16-byte aligned.  Elements behind rot are copied.  q of a token without a position (padding, or
+ * outside its sequence's pages) is copied as it is.  nh = 0: no q.  cu_q NULL: one token a
+ * sequence, N = B. */
+int cta_paged_kv_append(
+    const float* q, const int64_t* q_strides, const float* k, const int64_t* k_strides,
+    const float* v, const int64_t* v_strides, int64_t N, int64_t nh, int64_t nkv, int64_t hs,
+    const float* cos, const float* sin, int64_t rot, int interleaved,
+    float* k_cache, const int64_t* k_cache_strides, float* v_cache, const int64_t* v_cache_strides,
+    int64_t num_pages, int64_t page_size, const int32_t* page_table, int64_t table_stride,
+    int64_t pages_per_seq, const int32_t* seq_lens, const int32_t* cu_q, int64_t B,
+    float* q_out, void* stream);
+int cta_paged_kv_append_bf16(
+    const uint16_t* q, const int64_t* q_strides, const uint16_t* k, const int64_t* k_strides,
+    const uint16_t* v, const int64_t* v_strides, int64_t N, int64_t nh, int64_t nkv, int64_t hs,
+    const float* cos, const float* sin, int64_t rot, int interleaved,
+    uint16_t* k_cache, const int64_t* k_cache_strides, uint16_t* v_cache, const int64_t* v_cache_strides,
+    int64_t num_pages, int64_t page_size, const int32_t* page_table, int64_t table_stride,
+    int64_t pages_per_seq, const int32_t* seq_lens, const int32_t* cu_q, int64_t B,
+    uint16_t* q_out, void* stream);
+int cta_paged_kv_append_f16(
+    const uint16_t* q, const int64_t* q_strides, const uint16_t* k, const int64_t* k_strides,
+    const uint16_t* v, const int64_t* v_strides, int64_t N, int64_t nh, int64_t nkv, int64_t hs,
+    const float* cos, const float* sin, int64_t rot, int interleaved,
+    uint16_t* k_cache, const int64_t* k_cache_strides, uint16_t* v_cache, const int64_t* v_cache_strides,
+    int64_t num_pages, int64_t page_size, const int32_t* page_table, int64_t table_stride,
+    int64_t pages_per_seq, const int32_t* seq_lens, const int32_t* cu_q, int64_t B,
+    uint16_t* q_out, void* stream);
+
+/* Attention of one new token a sequence: q (B, nh, hs) at position seq_lens[b] - 1, nh a multiple
+ * of nkv, query head h reading key/value head h / (nh / nkv).  O (B, nh, hs) and L (B, nh) dense,
+ * L = rowmax + ln(rowsum) of scale q.k; a row without a key gives O = 0, L = -inf.  The workspace
+ * (cta_paged_attention_decode_workspace bytes, 16-byte aligned) holds partial results; it needs no
+ * initialisation and must not be shared by calls that may overlap. */
+int64_t cta_paged_attention_decode_workspace(int64_t B, int64_t nh, int64_t nkv, int64_t hs,
+                                             int64_t pages_per_seq, int64_t page_size);
+int cta_paged_attention_decode(
+    const float* q, const int64_t* q_strides,
+    const float* k_cache, const int64_t* k_cache_strides,
+    const float* v_cache, const int64_t* v_cache_strides, int64_t num_pages, int64_t page_size,
+    const int32_t* page_table, int64_t table_stride, int64_t pages_per_seq,
+    const int32_t* seq_lens, int64_t B, int64_t nh, int64_t nkv, int64_t hs, float scale,
+    float* o, float* l, void* workspace, int64_t workspace_bytes, void* stream);
+int cta_paged_attention_decode_bf16(
+    const uint16_t* q, const int64_t* q_strides,
+    const uint16_t* k_cache, const int64_t* k_cache_strides,
+    const uint16_t* v_cache, const int64_t* v_cache_strides, int64_t num_pages, int64_t page_size,
+    const int32_t* page_table, int64_t table_stride, int64_t pages_per_seq,
+    const int32_t* seq_lens, int64_t B, int64_t nh, int64_t nkv, int64_t hs, float scale,
+    uint16_t* o, float* l, void* workspace, int64_t workspace_bytes, void* stream);
+int cta_paged_attention_decode_f16(
+    const uint16_t* q, const int64_t* q_strides,
+    const uint16_t* k_cache, const int64_t* k_cache_strides,
+    const uint16_t* v_cache, const int64_t* v_cache_strides, int64_t num_pages, int64_t page_size,
+    const int32_t* page_table, int64_t table_stride, int64_t pages_per_seq,
+    const int32_t* seq_lens, int64_t B, int64_t nh, int64_t nkv, int64_t hs, float scale,
+    uint16_t* o, float* l, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Attention of packed new tokens: q (N, nh, hs), each token seeing its sequence's positions up to
+ * its own.  O (N, nh, hs) and L (N, nh) as above; padding rows give O = 0, L = -inf. */
+int64_t cta_paged_attention_prefill_workspace(int64_t B, int64_t N, int64_t nh, int64_t nkv,
+                                              int64_t hs, int64_t pages_per_seq,
+                                              int64_t page_size);
+int cta_paged_attention_prefill(
+    const float* q, const int64_t* q_strides,
+    const float* k_cache, const int64_t* k_cache_strides,
+    const float* v_cache, const int64_t* v_cache_strides, int64_t num_pages, int64_t page_size,
+    const int32_t* page_table, int64_t table_stride, int64_t pages_per_seq,
+    const int32_t* seq_lens, const int32_t* cu_q, int64_t B, int64_t N, int64_t nh, int64_t nkv,
+    int64_t hs, float scale, float* o, float* l, void* workspace, int64_t workspace_bytes,
+    void* stream);
+int cta_paged_attention_prefill_bf16(
+    const uint16_t* q, const int64_t* q_strides,
+    const uint16_t* k_cache, const int64_t* k_cache_strides,
+    const uint16_t* v_cache, const int64_t* v_cache_strides, int64_t num_pages, int64_t page_size,
+    const int32_t* page_table, int64_t table_stride, int64_t pages_per_seq,
+    const int32_t* seq_lens, const int32_t* cu_q, int64_t B, int64_t N, int64_t nh, int64_t nkv,
+    int64_t hs, float scale, uint16_t* o, float* l, void* workspace, int64_t workspace_bytes,
+    void* stream);
+int cta_paged_attention_prefill_f16(
+    const uint16_t* q, const int64_t* q_strides,
+    const uint16_t* k_cache, const int64_t* k_cache_strides,
+    const uint16_t* v_cache, const int64_t* v_cache_strides, int64_t num_pages, int64_t page_size,
+    const int32_t* page_table, int64_t table_stride, int64_t pages_per_seq,
+    const int32_t* seq_lens, const int32_t* cu_q, int64_t B, int64_t N, int64_t nh, int64_t nkv,
+    int64_t hs, float scale, uint16_t* o, float* l, void* workspace, int64_t workspace_bytes,
+    void* stream);
 
 #ifdef __cplusplus
 }

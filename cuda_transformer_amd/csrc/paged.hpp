@@ -84,5 +84,8 @@ struct PagedArgs {
 int check_paged(const PagedArgs& a, int elem, PagedPlan& plan);
 // Packed tokens: strides (token, head, d) with 16-byte rows.
 bool tokens_layout_ok(const void* p, const int64_t* s, int elem);
+// Validates what the attention entries take besides: queries, results, the scale.
+int check_paged_rows(const void* q, const int64_t* qs, int64_t rows, const PagedArgs& a, float scale,
+                     const void* o, const float* l, int elem, const char* what);
 
 }  // namespace cta

@@ -27,8 +27,9 @@ int check_paged(const PagedArgs& a, int elem, PagedPlan& plan) {
   const int64_t vec = 16 / elem;
   for (const int64_t* s : {a.ks, a.vs})
     if (!s || s[3] != 1 || s[0] % vec || s[1] % vec || s[2] % vec || s[0] < 0 || s[1] < 0 ||
-        s[2] < 0)
-      return fail(CTA_ERR_LAYOUT, "the caches need a unit last stride and 16-byte rows");
+        s[2] < 0 || s[2] >= (int64_t)1 << 24)
+      return fail(CTA_ERR_LAYOUT,
+                  "the caches need a unit last stride, 16-byte rows and row strides below 2^24");
   if (a.num_pages > 0 && (!a.k_cache || !a.v_cache || !aligned16(a.k_cache) || !aligned16(a.v_cache)))
     return fail(CTA_ERR_LAYOUT, "the caches need 16-byte aligned bases");
   plan.table = a.page_table;
@@ -37,7 +38,7 @@ int check_paged(const PagedArgs& a, int elem, PagedPlan& plan) {
   plan.cu_q = a.cu_q;
   plan.B = (int)a.B;
   plan.num_pages = (int)a.num_pages;
-  plan.capacity = (int)(a.pages_per_seq * a.page_size);
+  plan.capacity = a.num_pages == 0 ? 0 : (int)(a.pages_per_seq * a.page_size);
   plan.ps = FastDiv((uint32_t)a.page_size);
   return CTA_OK;
 }
@@ -46,6 +47,19 @@ bool tokens_layout_ok(const void* p, const int64_t* s, int elem) {
   const int64_t vec = 16 / elem;
   return p != nullptr && s != nullptr && aligned16(p) && s[2] == 1 && s[0] % vec == 0 &&
          s[1] % vec == 0;
+}
+
+int check_paged_rows(const void* q, const int64_t* qs, int64_t rows, const PagedArgs& a, float scale,
+                     const void* o, const float* l, int elem, const char* what) {
+  if (rows < 0 || rows > (int64_t)1 << 24 || rows * a.nh > (int64_t)1 << 30)
+    return fail(CTA_ERR_INVALID_ARGUMENT, "size too large");
+  if (!std::isfinite(scale)) return fail(CTA_ERR_INVALID_ARGUMENT, "scale must be finite");
+  if (rows * a.nh == 0) return CTA_OK;
+  if (!o || !l) return fail(CTA_ERR_INVALID_ARGUMENT, "null output pointer");
+  if (!tokens_layout_ok(q, qs, elem) || !aligned16(o))
+    return fail(CTA_ERR_LAYOUT,
+                std::string(what) + " needs dense heads in 16-byte aligned rows (q, o)");
+  return CTA_OK;
 }
 
 namespace {
@@ -123,14 +137,8 @@ int attention(const P* q, const int64_t* qs, int64_t rows, float scale, P* o, fl
               const PagedArgs& pa, void* stream, const char* what) {
   PagedPlan plan;
   if (int rc = check_paged(pa, sizeof(E), plan)) return rc;
-  if (rows < 0 || rows > (int64_t)1 << 24 || rows * pa.nh > (int64_t)1 << 30)
-    return fail(CTA_ERR_INVALID_ARGUMENT, "size too large");
-  if (!std::isfinite(scale)) return fail(CTA_ERR_INVALID_ARGUMENT, "scale must be finite");
+  if (int rc = check_paged_rows(q, qs, rows, pa, scale, o, l, sizeof(E), what)) return rc;
   if (rows * pa.nh == 0) return CTA_OK;
-  if (!o || !l) return fail(CTA_ERR_INVALID_ARGUMENT, "null output pointer");
-  if (!tokens_layout_ok(q, qs, sizeof(E)) || !aligned16(o))
-    return fail(CTA_ERR_LAYOUT,
-                std::string(what) + " needs dense heads in 16-byte aligned rows (q, o)");
   AttnArgs<E> a;
   a.q = reinterpret_cast<const E*>(q);
   a.k = static_cast<const E*>(pa.k_cache); a.v = static_cast<const E*>(pa.v_cache);
@@ -154,18 +162,6 @@ int attention(const P* q, const int64_t* qs, int64_t rows, float scale, P* o, fl
 using namespace cta;
 
 #define CTA_PAGED_ATTENTION(NAME_SUFFIX, TYPE, PTR)                                               \
-  extern "C" int cta_paged_attention_decode##NAME_SUFFIX(                                         \
-      const PTR* q, const int64_t* q_strides, const PTR* k_cache, const int64_t* k_cache_strides, \
-      const PTR* v_cache, const int64_t* v_cache_strides, int64_t num_pages, int64_t page_size,   \
-      const int32_t* page_table, int64_t table_stride, int64_t pages_per_seq,                     \
-      const int32_t* seq_lens, int64_t B, int64_t nh, int64_t nkv, int64_t hs, float scale,       \
-      PTR* o, float* l, void* workspace, int64_t workspace_bytes, void* stream) {                 \
-    return attention<TYPE>(q, q_strides, B, scale, o, l,                                          \
-                           {k_cache_strides, v_cache_strides, num_pages, page_size, table_stride, \
-                            pages_per_seq, B, nh, nkv, hs, page_table, seq_lens, nullptr,         \
-                            k_cache, v_cache},                                                    \
-                           stream, "paged_attention_decode");                                     \
-  }                                                                                               \
   extern "C" int cta_paged_attention_prefill##NAME_SUFFIX(                                        \
       const PTR* q, const int64_t* q_strides, const PTR* k_cache, const int64_t* k_cache_strides, \
       const PTR* v_cache, const int64_t* v_cache_strides, int64_t num_pages, int64_t page_size,   \
@@ -185,10 +181,6 @@ CTA_PAGED_ATTENTION(_bf16, __bf16, uint16_t)
 CTA_PAGED_ATTENTION(_f16, _Float16, uint16_t)
 #undef CTA_PAGED_ATTENTION
 
-extern "C" int64_t cta_paged_attention_decode_workspace(int64_t, int64_t, int64_t, int64_t, int64_t,
-                                                        int64_t) {
-  return 0;
-}
 extern "C" int64_t cta_paged_attention_prefill_workspace(int64_t, int64_t, int64_t, int64_t, int64_t,
                                                          int64_t, int64_t) {
   return 0;

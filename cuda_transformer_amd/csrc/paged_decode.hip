@@ -1,0 +1,606 @@
+// Attention of one new token a sequence over a paged key/value cache, its length split over the GPU.
+//
+// Query head h of sequence b reads key/value head h / group; over the sequence's keys j < seq_lens[b]
+// whose page is mapped, in exponents of 2 (t_j = scale log2(e) q . k_j):
+//   m = max t,  l = sum 2^{t_j - m},  O = sum 2^{t_j - m} v_j / l,  L = (m + log2 l) ln 2;
+// without a key O = 0, L = -inf.  Any cut of the keys gives parts (m_i, l_i, O_i l_i) that add up
+// against the largest m_i.
+//
+// What bounds it: every key and value is read once, 2 group to 4 group operations a byte.  So the
+// products run on the matrix pipe, whose idle columns cost nothing (16 query heads a pass, whatever
+// the group), and everything else serves the loads.
+//  * A job is one sequence's keys for one key/value head (and 16 of its query heads).  Jobs are cut
+//    into tiles of 4 x WK keys and all tiles of all jobs are dealt evenly, in order, to a fixed
+//    number of workgroups: lengths that differ by any factor load the GPU evenly.  A workgroup
+//    writes the jobs it has whole, and partial results (at most two: the job it enters in the
+//    middle, and the job it leaves) to the workspace, which a second kernel joins in tile order.
+//    Both recompute the deal from seq_lens, so the host never looks at the lengths.
+//  * A wave takes WK keys of each tile.  K goes from memory to registers in the order of the MFMA's
+//    A operand (row = key): lane l, key l % 16, 16 bytes at 64 s + 16 (l / 16) for step s.  The
+//    scores come back with four keys of one head in a lane: S[key 4 (l / 16) + r][head l % 16].
+//  * V: lane l reads, for the keys whose scores it holds, elements (HS / 16) (l % 16) .. of the row
+//    (16 lanes read a whole row), and turns them in registers (one v_perm a pair of values) into the
+//    A operand of O^T += V^T P^T: MFMA e has rows d = (HS / 16) c + e.  The lane's probabilities are
+//    the B operand as they are.  No LDS, no shuffle of K, V or P, and both products' loads are
+//    issued a tile ahead.
+//  * Probabilities are kept to two 16-bit parts for the 16-bit types (the second product is free
+//    beside the loads): rounding them once would add as much error as the output's own rounding.
+//  * FP32 runs on the FP32 MFMA (16x16x4).
+#include "paged.hpp"
+
+namespace cta {
+namespace {
+
+template <class E>
+struct DecodeArgs {
+  const E *q, *k, *v;
+  int64_t qt, qh;
+  Strides3 sk, sv;
+  int nh, nkv, group, chunks;  // chunks of 16 query heads a key/value head
+  float scale_log2;
+  E* o;
+  float* l;
+  float* ws;
+};
+
+// Geometry of a type and head size: 16 KB of K and V a wave and tile.
+template <class E, int HS>
+struct DecodeTile {
+  static constexpr int KG = sizeof(E) == 2 ? 256 / HS : 128 / HS;  // groups of 16 keys a wave
+  static constexpr int WK = 16 * KG;                               // keys a wave
+  static constexpr int TILE = 4 * WK;
+  static constexpr int CK = HS * (int)sizeof(E) / 64;  // 16-byte chunks a lane has of a K row
+  static constexpr int DW = HS * (int)sizeof(E) / 64;  // dwords a lane has of a V row
+  static constexpr int NE = HS / 16;                   // output elements of a lane and register
+  static constexpr int PART = 16 * (HS + 2);           // floats of a partial result: O, m, l
+};
+
+// Largest of the values that lanes l, l ^ 16, l ^ 32, l ^ 48 hold, and their sum.
+__device__ __forceinline__ float max_quarters(float v) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return max_halves(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
+}
+__device__ __forceinline__ float sum_quarters(float v) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return sum_halves(__uint_as_float(r[0]) + __uint_as_float(r[1]));
+}
+
+__device__ __forceinline__ f32x4 mfma16(vec8_t<__bf16> a, vec8_t<__bf16> b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mfma16(vec8_t<_Float16> a, vec8_t<_Float16> b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mfma16(float a, float b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
+}
+
+// Tiles of sequence b.
+template <int TILE>
+__device__ __forceinline__ int tiles_of(const PagedPlan& plan, int b) {
+  return (plan.keys_to((int64_t)plan.lens[b] - 1) + TILE - 1) / TILE;
+}
+// Sum of the lanes' values below this lane, and (all) of the wave.
+__device__ __forceinline__ int64_t wave_scan(int64_t v, int64_t& all) {
+  const int lane = threadIdx.x & 63;
+  int64_t s = v;
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const int64_t o = __shfl_up(s, off);
+    if (lane >= off) s += o;
+  }
+  all = __shfl(s, 63);
+  return s - v;
+}
+// Tiles of all sequences (one job each); before: those of the sequences in front of b.
+template <int TILE>
+__device__ __forceinline__ int64_t count_tiles(const PagedPlan& plan, int b, int64_t& before) {
+  const int lane = threadIdx.x & 63;
+  int64_t total = 0, front = 0;
+  for (int i = lane; i - lane < plan.B; i += 64) {
+    const int64_t n = i < plan.B ? tiles_of<TILE>(plan, i) : 0;
+    total += n;
+    if (i < b) front += n;
+  }
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) {
+    total += __shfl_xor(total, off);
+    front += __shfl_xor(front, off);
+  }
+  before = front;
+  return total;
+}
+// Sequence that holds tile x of the sequences' tiles in a row (x < their number); before as above.
+template <int TILE>
+__device__ __forceinline__ int find_tile(const PagedPlan& plan, int64_t x, int64_t& before) {
+  const int lane = threadIdx.x & 63;
+  int64_t base = 0;
+  for (int i = lane; i - lane < plan.B; i += 64) {
+    const int64_t n = i < plan.B ? tiles_of<TILE>(plan, i) : 0;
+    int64_t all;
+    const int64_t at = base + wave_scan(n, all);
+    const uint64_t hit = __ballot(x >= at && x < at + n);
+    if (hit) {
+      const int w = __ffsll((unsigned long long)hit) - 1;
+      before = __shfl(at, w);
+      return i - lane + w;
+    }
+    base += all;
+  }
+  before = base;
+  return plan.B;
+}
+// First unit of workgroup w of W <= units: each has at least one.
+__device__ __forceinline__ int64_t deal_start(int64_t units, int w, int W) { return units * w / W; }
+
+template <class E, int HS, bool UNIFORM>
+__global__ __launch_bounds__(256, 2) void paged_decode_kernel(DecodeArgs<E> a, PagedPlan plan,
+                                                              bool direct) {
+  using D = DecodeTile<E, HS>;
+  constexpr int KG = D::KG, WK = D::WK, TILE = D::TILE, CK = D::CK, DW = D::DW, NE = D::NE;
+  constexpr bool F32 = sizeof(E) == 4;
+  constexpr int OP = HS + 4;  // pitch of a head's row in the exchange
+  __shared__ __attribute__((aligned(16))) float xo[4][16][OP];
+  __shared__ float xm[4][16], xl[4][16];
+  __shared__ int64_t rows_at[UNIFORM ? 1 : 4][2][UNIFORM ? 1 : WK];
+
+  const int lane = threadIdx.x & 63, wave = wave_index();
+  const int col = lane & 15, quarter = lane >> 4;
+  const int jobs = a.nkv * a.chunks;  // jobs a sequence
+
+  int64_t u = 0, u_end = 0;
+  int b, job, t, n_tiles;
+  if (direct) {
+    b = blockIdx.x / jobs;
+    job = blockIdx.x - b * jobs;
+    t = 0;
+    n_tiles = tiles_of<TILE>(plan, b);
+    u_end = n_tiles;
+  } else {
+    int64_t before;
+    const int64_t units = count_tiles<TILE>(plan, 0, before) * jobs;
+    const int W = (int)min(units, (int64_t)gridDim.x);
+    if ((int)blockIdx.x >= W) return;
+    u = deal_start(units, blockIdx.x, W);
+    u_end = deal_start(units, blockIdx.x + 1, W);
+    b = find_tile<TILE>(plan, u / jobs, before);
+    n_tiles = tiles_of<TILE>(plan, b);
+    const int64_t in_seq = u - before * jobs;
+    job = (int)(in_seq / n_tiles);
+    t = (int)(in_seq - (int64_t)job * n_tiles);
+  }
+
+  for (;;) {
+    // ---- one job, tiles [t, t_end)
+    const int t_end = (int)min((int64_t)n_tiles, t + (u_end - u));
+    const int keys = plan.keys_to((int64_t)plan.lens[b] - 1);
+    const int kvh = job / a.chunks, chunk = job - kvh * a.chunks;
+    const int head0 = kvh * a.group + 16 * chunk, heads = min(16, a.group - 16 * chunk);
+    const int32_t* table = plan.table + b * plan.table_stride;
+    const E* kb = a.k + kvh * a.sk.h;
+    const E* vb = a.v + kvh * a.sv.h;
+
+    // Q in the order of the B operand: column = head, the chunk of d of the K operand
+    u32x4 qf[CK];
+#pragma unroll
+    for (int s = 0; s < CK; ++s) {
+      qf[s] = u32x4{0, 0, 0, 0};
+      if (col < heads)
+        qf[s] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const char*>(
+                    a.q + b * a.qt + (head0 + col) * a.qh) + 64 * s + 16 * quarter);
+    }
+
+    f32x4 acc[NE];
+#pragma unroll
+    for (int e = 0; e < NE; ++e) acc[e] = f32x4{0, 0, 0, 0};
+    float m = -INFINITY, l = 0.0f;
+
+    // Page of this wave's group of 16 keys (UNIFORM): lane i has group i % KG of the i / KG-th tile
+    // from tp on.  Entries behind the last key are not read.
+    constexpr int TP = 64 / KG;  // tiles that a load of pages covers
+    auto load_pages = [&](int tp) {
+      const int key = (tp + lane / KG) * TILE + wave * WK + 16 * (lane % KG);
+      int page = -1;
+      if (key < keys && tp + lane / KG < t_end) {
+        page = table[plan.ps.div(key)];
+        page = (uint32_t)page < (uint32_t)plan.num_pages ? page : -1;
+      }
+      return page;
+    };
+    int tp = t, pages = -1, pages_next = -1;
+    if constexpr (UNIFORM) {
+      pages = load_pages(tp);
+      pages_next = load_pages(tp + TP);
+    }
+
+    u32x4 kr[KG][CK];
+    uint32_t vr[4 * KG][DW];
+    uint32_t valid_k = 0, valid_v = 0;  // bit 4 g + r: key 16 g + 4 quarter + r of the tile in kr, vr
+    bool full_k = false, full_v = false;
+    int page_of[KG];  // of the tile whose K was loaded last (UNIFORM)
+
+    auto load_k = [&](int tile) {
+      const int k0 = tile * TILE + wave * WK;
+      if constexpr (UNIFORM) {
+        if (tile - tp >= TP) {
+          tp += TP;
+          pages = pages_next;
+          pages_next = load_pages(tp + TP);
+        }
+        full_k = k0 + WK <= keys;
+#pragma unroll
+        for (int g = 0; g < KG; ++g) {
+          page_of[g] = __builtin_amdgcn_readlane(pages, (tile - tp) * KG + g);
+          full_k = full_k && page_of[g] >= 0;
+        }
+        valid_k = 0;
+#pragma unroll
+        for (int g = 0; g < KG; ++g) {
+          const int key = k0 + 16 * g;
+          const int row = key - plan.ps.div(key) * (int)plan.ps.d;
+          // an unmapped group reads page 0; nothing of it is used
+          const E* p = kb + max(page_of[g], 0) * a.sk.a + row * a.sk.r;
+          const int at = col * (int)a.sk.r * (int)sizeof(E) + 16 * quarter;
+#pragma unroll
+          for (int s = 0; s < CK; ++s)
+            kr[g][s] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const char*>(p) + (uint32_t)(at + 64 * s));
+          if (page_of[g] >= 0)
+            valid_k |= (0xfu >> (4 - min(max(keys - key - 4 * quarter, 0), 4))) << (4 * g);
+        }
+      } else {
+        // offsets of the tile's rows, one a lane, through this wave's part of LDS; -1: no key
+        wave_lds_fence();
+#pragma unroll
+        for (int i = 0; i < (WK + 63) / 64; ++i) {
+          const int j = lane + 64 * i, key = k0 + j;
+          int page = -1, row = 0;
+          if (key < keys) {
+            const int at = plan.ps.div(key);
+            row = key - at * (int)plan.ps.d;
+            page = table[at];
+          }
+          const bool ok = (uint32_t)page < (uint32_t)plan.num_pages;
+          if (j < WK) {
+            rows_at[wave][0][j] = ok ? page * a.sk.a + row * a.sk.r : -1;
+            rows_at[wave][1][j] = ok ? page * a.sv.a + row * a.sv.r : -1;
+          }
+        }
+        wave_lds_fence();
+        valid_k = 0;
+#pragma unroll
+        for (int g = 0; g < KG; ++g) {
+          const int64_t at = max(rows_at[wave][0][16 * g + col], (int64_t)0);
+#pragma unroll
+          for (int s = 0; s < CK; ++s)
+            kr[g][s] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const char*>(kb + at) + 64 * s + 16 * quarter);
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            valid_k |= (uint32_t)(rows_at[wave][0][16 * g + 4 * quarter + r] >= 0) << (4 * g + r);
+        }
+        full_k = __all(valid_k == (uint32_t)((1ull << (4 * KG)) - 1));
+      }
+    };
+    auto load_v = [&](int tile) {  // of the tile whose K was loaded last
+      valid_v = valid_k;
+      full_v = full_k;
+#pragma unroll
+      for (int g = 0; g < KG; ++g) {
+        const E* p = vb;
+        if constexpr (UNIFORM) {
+          const int key = tile * TILE + wave * WK + 16 * g;
+          const int row = key - plan.ps.div(key) * (int)plan.ps.d;
+          p = vb + max(page_of[g], 0) * a.sv.a + row * a.sv.r;
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const char* src;
+          if constexpr (UNIFORM) {
+            src = reinterpret_cast<const char*>(p) +
+                  (uint32_t)((4 * quarter + r) * (int)a.sv.r * (int)sizeof(E) + col * DW * 4);
+          } else {
+            const int64_t at = max(rows_at[wave][1][16 * g + 4 * quarter + r], (int64_t)0);
+            src = reinterpret_cast<const char*>(vb + at) + col * DW * 4;
+          }
+          uint32_t(&x)[DW] = vr[4 * g + r];
+          if constexpr (DW >= 4) {
+#pragma unroll
+            for (int c = 0; c < DW / 4; ++c) {
+              const u32x4 w = reinterpret_cast<const u32x4*>(src)[c];
+#pragma unroll
+              for (int i = 0; i < 4; ++i) x[4 * c + i] = w[i];
+            }
+          } else if constexpr (DW == 2) {
+            const uint2 w = *reinterpret_cast<const uint2*>(src);
+            x[0] = w.x; x[1] = w.y;
+          } else {
+            x[0] = *reinterpret_cast<const uint32_t*>(src);
+          }
+        }
+      }
+    };
+
+    if (t < t_end) {
+      load_k(t);
+      load_v(t);
+    }
+    for (int tile = t; tile < t_end; ++tile) {
+      // ---- scores of 16 KG keys: lane, register r of group g: key 16 g + 4 quarter + r, head col
+      f32x4 s[KG];
+#pragma unroll
+      for (int g = 0; g < KG; ++g) s[g] = f32x4{0, 0, 0, 0};
+#pragma unroll
+      for (int c = 0; c < CK; ++c)
+#pragma unroll
+        for (int g = 0; g < KG; ++g) {
+          if constexpr (F32) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              s[g] = mfma16(__uint_as_float(kr[g][c][i]), __uint_as_float(qf[c][i]), s[g]);
+          } else {
+            s[g] = mfma16(__builtin_bit_cast(vec8_t<E>, kr[g][c]), __builtin_bit_cast(vec8_t<E>, qf[c]), s[g]);
+          }
+        }
+      if (tile + 1 < t_end) load_k(tile + 1);
+      float mt = -INFINITY;
+#pragma unroll
+      for (int g = 0; g < KG; ++g)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          s[g][r] *= a.scale_log2;
+          if (!full_v && !(valid_v >> (4 * g + r) & 1)) s[g][r] = -INFINITY;
+          mt = fmaxf(mt, s[g][r]);
+        }
+      mt = max_quarters(mt);
+      if (__any(mt > m)) {
+        const float m_new = fmaxf(m, mt);
+        const float alpha = fast_exp2(m - (m_new == -INFINITY ? 0.0f : m_new));
+        l *= alpha;
+#pragma unroll
+        for (int e = 0; e < NE; ++e) acc[e] *= alpha;
+        m = m_new;
+      }
+      const float off = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+      for (int g = 0; g < KG; ++g)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          s[g][r] = fast_exp2(s[g][r] - off);
+          l += s[g][r];
+        }
+      // rows without a key count as zeros: what lies there may be anything
+      if (!full_v) {
+#pragma unroll
+        for (int i = 0; i < 4 * KG; ++i)
+          if (!(valid_v >> i & 1)) {
+#pragma unroll
+            for (int w = 0; w < DW; ++w) vr[i][w] = 0;
+          }
+      }
+      // ---- O^T += V^T P^T
+      if constexpr (F32) {
+#pragma unroll
+        for (int g = 0; g < KG; ++g)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int e = 0; e < NE; ++e)
+              acc[e] = mfma16(__uint_as_float(vr[4 * g + r][e]), s[g][r], acc[e]);
+      } else {
+#pragma unroll
+        for (int g = 0; g < KG; g += 2) {  // 32 keys: the lane's 8 are its k-slots
+          vec8_t<E> hi, lo;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const float p = s[g + (j >> 2)][j & 3];
+            hi[j] = (E)p;
+            lo[j] = (E)(p - (float)hi[j]);
+          }
+#pragma unroll
+          for (int e = 0; e < NE; ++e) {
+            u32x4 w;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const uint32_t x = vr[4 * g + 2 * i][e / 2], y = vr[4 * g + 2 * i + 1][e / 2];
+              w[i] = e % 2 ? pack_hi16(x, y) : pack_lo16(x, y);
+            }
+            const auto va = __builtin_bit_cast(vec8_t<E>, w);
+            acc[e] = mfma16(va, lo, acc[e]);
+            acc[e] = mfma16(va, hi, acc[e]);
+          }
+        }
+      }
+      if (tile + 1 < t_end) load_v(tile + 1);
+    }
+
+    // ---- the four waves' parts, against the largest offset
+    l = sum_quarters(l);
+    if (quarter == 0) { xm[wave][col] = m; xl[wave][col] = l; }
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+      for (int e = 0; e < NE; ++e) xo[wave][col][NE * (4 * quarter + r) + e] = acc[e][r];
+    __syncthreads();
+    const bool whole = t == 0 && t_end == n_tiles;
+    // a job that began in an earlier workgroup goes to this one's first slot, else to its second
+    float* part = a.ws + ((int64_t)blockIdx.x * 2 + (t == 0)) * D::PART;
+    constexpr int TPH = HS / 4;  // threads a head
+    for (int h = threadIdx.x / TPH; h < heads; h += 256 / TPH) {
+      const int d = 4 * (threadIdx.x % TPH);
+      float mj = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) mj = fmaxf(mj, xm[w][h]);
+      const float off = mj == -INFINITY ? 0.0f : mj;
+      float lj = 0.0f;
+      float4 o = zero4();
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const float f = fast_exp2(xm[w][h] - off);
+        const float4 x = ld4(&xo[w][h][d]);
+        lj = fmaf(f, xl[w][h], lj);
+        o.x = fmaf(f, x.x, o.x); o.y = fmaf(f, x.y, o.y);
+        o.z = fmaf(f, x.z, o.z); o.w = fmaf(f, x.w, o.w);
+      }
+      if (whole) {
+        const float inv = lj == 0.0f ? 0.0f : 1.0f / lj;
+        const int64_t at = (int64_t)b * a.nh + head0 + h;
+        E* op = a.o + at * HS + d;
+        op[0] = (E)(o.x * inv); op[1] = (E)(o.y * inv);
+        op[2] = (E)(o.z * inv); op[3] = (E)(o.w * inv);
+        if (d == 0) a.l[at] = lj == 0.0f ? -INFINITY : off * kLn2 + logf(lj);
+      } else {
+        st4(part + h * HS + d, o);
+        if (d == 0) { part[16 * HS + h] = mj; part[16 * HS + 16 + h] = lj; }
+      }
+    }
+
+    u += t_end - t;
+    if (direct || u >= u_end) return;
+    __syncthreads();  // the exchange is read: the next job may write it
+    t = 0;
+    if (++job == jobs) {
+      job = 0;
+      do n_tiles = tiles_of<TILE>(plan, ++b); while (n_tiles == 0);
+    }
+  }
+}
+
+// Joins the parts of the jobs that several workgroups of W share; rows without a key.  One workgroup
+// for each sequence and query head; its threads take an element of the row and every PG-th part.
+template <class E, int HS>
+__global__ __launch_bounds__(256) void paged_decode_join_kernel(DecodeArgs<E> a, PagedPlan plan,
+                                                                int grid) {
+  using D = DecodeTile<E, HS>;
+  constexpr int PG = 256 / HS;
+  __shared__ float xo[PG][HS], xl[PG];
+  const int b = blockIdx.x / a.nh, h = blockIdx.x - b * a.nh;
+  const int kvh = h / a.group, in_group = h - kvh * a.group;
+  const int job = kvh * a.chunks + in_group / 16, row = in_group % 16;
+  const int jobs = a.nkv * a.chunks;
+  int64_t before;
+  const int64_t units = count_tiles<D::TILE>(plan, b, before) * jobs;
+  const int n = tiles_of<D::TILE>(plan, b);
+  const int64_t at = (int64_t)b * a.nh + h;
+  const int d = threadIdx.x % HS, pg = threadIdx.x / HS;
+  if (n == 0) {
+    if (pg == 0) a.o[at * HS + d] = (E)0.0f;
+    if (threadIdx.x == 0) a.l[at] = -INFINITY;
+    return;
+  }
+  const int W = (int)min(units, (int64_t)grid);
+  // workgroups of the job's first and last unit: the last w with deal_start(w) <= unit
+  const int64_t first = before * jobs + (int64_t)job * n, last = first + n - 1;
+  auto owner = [&](int64_t unit) { return (int)(((unit + 1) * W - 1) / units); };
+  const int w0 = owner(first), w1 = owner(last);
+  if (w0 == w1) return;  // written whole
+  auto part = [&](int w) { return a.ws + ((int64_t)w * 2 + (w == w0)) * D::PART; };
+
+  const int lane = threadIdx.x & 63;
+  float m = -INFINITY;
+  for (int w = w0 + lane; w <= w1; w += 64) m = fmaxf(m, part(w)[16 * HS + row]);
+  m = wave_max(m);
+  const float off = m == -INFINITY ? 0.0f : m;
+  float o = 0.0f, l = 0.0f;
+  for (int w = w0 + pg; w <= w1; w += PG) {
+    const float* p = part(w);
+    const float f = fast_exp2(p[16 * HS + row] - off);
+    l = fmaf(f, p[16 * HS + 16 + row], l);
+    o = fmaf(f, p[row * HS + d], o);
+  }
+  xo[pg][d] = o;
+  if (d == 0) xl[pg] = l;
+  __syncthreads();
+  if (pg != 0) return;
+#pragma unroll
+  for (int i = 1; i < PG; ++i) { o += xo[i][d]; l += xl[i]; }
+  a.o[at * HS + d] = (E)(l == 0.0f ? 0.0f : o / l);
+  if (d == 0) a.l[at] = l == 0.0f ? -INFINITY : off * kLn2 + logf(l);
+}
+
+// Workgroups that the tiles are dealt to, or 0 where every job is one workgroup's (direct).
+struct DecodeGrid {
+  int64_t jobs;
+  int W;
+};
+int tile_keys(int64_t hs, int elem) { return (int)(4 * 16 * (elem == 2 ? 256 / hs : 128 / hs)); }
+DecodeGrid decode_grid(int64_t B, int64_t nh, int64_t nkv, int64_t hs, int64_t capacity, int elem) {
+  DecodeGrid g;
+  g.jobs = B * nkv * ((nh / nkv + 15) / 16);
+  const int64_t tiles = (capacity + tile_keys(hs, elem) - 1) / tile_keys(hs, elem);
+  // Up to four tiles a job are walked in the time that the second kernel takes.
+  g.W = tiles <= 4 ? 0 : (int)std::min<int64_t>(g.jobs * tiles, 512);
+  return g;
+}
+
+template <class E, int HS>
+void launch_decode(const DecodeArgs<E>& a, const PagedPlan& plan, const DecodeGrid& g, hipStream_t st) {
+  const dim3 grid((unsigned)(g.W > 0 ? g.W : g.jobs));
+  if (plan.ps.d % 16 == 0)
+    hipLaunchKernelGGL((paged_decode_kernel<E, HS, true>), grid, dim3(256), 0, st, a, plan, g.W == 0);
+  else
+    hipLaunchKernelGGL((paged_decode_kernel<E, HS, false>), grid, dim3(256), 0, st, a, plan, g.W == 0);
+  if (g.W > 0)
+    hipLaunchKernelGGL((paged_decode_join_kernel<E, HS>), dim3((unsigned)(plan.B * a.nh)), dim3(256), 0, st, a, plan, g.W);
+}
+
+template <class E, class P>
+int decode(const P* q, const int64_t* qs, float scale, P* o, float* l, void* ws, int64_t ws_bytes,
+           const PagedArgs& pa, void* stream) {
+  PagedPlan plan;
+  if (int rc = check_paged(pa, sizeof(E), plan)) return rc;
+  if (int rc = check_paged_rows(q, qs, pa.B, pa, scale, o, l, sizeof(E), "paged_attention_decode"))
+    return rc;
+  if (pa.B * pa.nh == 0) return CTA_OK;
+  const DecodeGrid g = decode_grid(pa.B, pa.nh, pa.nkv, pa.hs, plan.capacity, sizeof(E));
+  if (g.W > 0 && (!ws || !aligned16(ws) ||
+                  ws_bytes < cta_paged_attention_decode_workspace(pa.B, pa.nh, pa.nkv, pa.hs,
+                                                                  pa.pages_per_seq, pa.page_size)))
+    return fail(CTA_ERR_INVALID_ARGUMENT, "paged_attention_decode needs its workspace");
+  DecodeArgs<E> a;
+  a.q = reinterpret_cast<const E*>(q);
+  a.k = static_cast<const E*>(pa.k_cache); a.v = static_cast<const E*>(pa.v_cache);
+  a.qt = qs[0]; a.qh = qs[1];
+  a.sk = {pa.ks[0], pa.ks[1], pa.ks[2]};
+  a.sv = {pa.vs[0], pa.vs[1], pa.vs[2]};
+  a.nh = (int)pa.nh; a.nkv = (int)pa.nkv; a.group = (int)(pa.nh / pa.nkv);
+  a.chunks = (a.group + 15) / 16;
+  a.scale_log2 = scale * kLog2e;
+  a.o = reinterpret_cast<E*>(o); a.l = l; a.ws = static_cast<float*>(ws);
+  const hipStream_t st = as_stream(stream);
+  if (pa.hs == 32) launch_decode<E, 32>(a, plan, g, st);
+  else if (pa.hs == 64) launch_decode<E, 64>(a, plan, g, st);
+  else launch_decode<E, 128>(a, plan, g, st);
+  return check_launch("paged_attention_decode");
+}
+
+}  // namespace
+}  // namespace cta
+
+using namespace cta;
+
+// The larger of what the types need: 16-bit tiles are the longer ones, FP32 has more of them.
+extern "C" int64_t cta_paged_attention_decode_workspace(int64_t B, int64_t nh, int64_t nkv,
+                                                        int64_t hs, int64_t pages_per_seq,
+                                                        int64_t page_size) {
+  if (B <= 0 || nh <= 0 || nkv <= 0 || pages_per_seq <= 0 || page_size <= 0 ||
+      (hs != 32 && hs != 64 && hs != 128) || pages_per_seq > ((int64_t)1 << 30) / page_size)
+    return 0;
+  return (int64_t)decode_grid(B, nh, nkv, hs, pages_per_seq * page_size, 4).W * 2 * 16 * (hs + 2) * 4;
+}
+
+#define CTA_PAGED_DECODE(SUFFIX, TYPE, PTR)                                                       \
+  extern "C" int cta_paged_attention_decode##SUFFIX(                                              \
+      const PTR* q, const int64_t* q_strides, const PTR* k_cache, const int64_t* k_cache_strides, \
+      const PTR* v_cache, const int64_t* v_cache_strides, int64_t num_pages, int64_t page_size,   \
+      const int32_t* page_table, int64_t table_stride, int64_t pages_per_seq,                     \
+      const int32_t* seq_lens, int64_t B, int64_t nh, int64_t nkv, int64_t hs, float scale,       \
+      PTR* o, float* l, void* workspace, int64_t workspace_bytes, void* stream) {                 \
+    return decode<TYPE>(q, q_strides, scale, o, l, workspace, workspace_bytes,                    \
+                        {k_cache_strides, v_cache_strides, num_pages, page_size, table_stride,    \
+                         pages_per_seq, B, nh, nkv, hs, page_table, seq_lens, nullptr, k_cache,   \
+                         v_cache},                                                                \
+                        stream);                                                                  \
+  }
+CTA_PAGED_DECODE(, float, float)
+CTA_PAGED_DECODE(_bf16, __bf16, uint16_t)
+CTA_PAGED_DECODE(_f16, _Float16, uint16_t)
+#undef CTA_PAGED_DECODE

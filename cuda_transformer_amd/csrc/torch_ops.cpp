@@ -862,8 +862,9 @@ void check_cache(const at::Tensor& c, const char* name, const at::Tensor& x) {
   const int64_t vec = 16 / c.element_size();
   const auto s = strides_of<4>(c);
   TORCH_CHECK((c.size(3) == 1 || c.stride(3) == 1) && s[0] % vec == 0 && s[1] % vec == 0 &&
-                  s[2] % vec == 0 && (reinterpret_cast<uintptr_t>(c.data_ptr()) & 15u) == 0,
-              name, " needs a unit last stride and 16-byte aligned rows");
+                  s[2] % vec == 0 && s[2] < ((int64_t)1 << 24) &&
+                  (reinterpret_cast<uintptr_t>(c.data_ptr()) & 15u) == 0,
+              name, " needs a unit last stride, 16-byte aligned rows and a row stride below 2^24");
 }
 
 struct PagedPlanTensors {

@@ -1,5 +1,5 @@
 // The paged key/value cache as its kernels see it: what is appended to it (paged_append.hip), and
-// the attention over it (paged_attention.hip).
+// the attention over it (paged_decode.hip, paged_prefill.hip).
 //
 // A cache is a pool of pages, (pages, kv heads, page size, hs).  Row b of the page table lists the
 // pages of sequence b in order: position p lies in page table[b][p / page size], row p % page size.
@@ -67,6 +67,53 @@ struct PagedPlan {
     return (int)min(max(p + 1, (int64_t)0), (int64_t)capacity);
   }
 };
+
+// Work counted in tiles, tiles(b) for sequence b: the host does not know the lengths, so a kernel
+// that shares it out counts them itself, 64 sequences a step.
+//
+// Tiles of all B sequences; before: those of the sequences in front of b.  For a whole wave.
+template <class F>
+__device__ __forceinline__ int64_t count_tiles(int B, int b, int64_t& before, F&& tiles) {
+  const int lane = threadIdx.x & 63;
+  int64_t total = 0, front = 0;
+  for (int i = lane; i < B; i += 64) {
+    const int64_t n = tiles(i);
+    total += n;
+    if (i < b) front += n;
+  }
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) {
+    total += __shfl_xor(total, off);
+    front += __shfl_xor(front, off);
+  }
+  before = front;
+  return total;
+}
+// Sequence that holds tile x of all tiles in a row, and the tiles before it; B, and all tiles, if
+// there are no more than x.  For a whole wave.
+template <class F>
+__device__ __forceinline__ int find_tile(int B, int64_t x, int64_t& before, F&& tiles) {
+  const int lane = threadIdx.x & 63;
+  before = 0;
+  for (int i0 = 0; i0 < B; i0 += 64) {
+    const int i = i0 + lane;
+    const int64_t n = i < B ? tiles(i) : 0;
+    int64_t end = n;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+      const int64_t o = __shfl_up(end, off);
+      if (lane >= off) end += o;
+    }
+    const uint64_t past = __ballot(before + end > x);
+    if (past) {
+      const int w = __ffsll((unsigned long long)past) - 1;
+      before += __shfl(end - n, w);
+      return i0 + w;
+    }
+    before += __shfl(end, 63);
+  }
+  return B;
+}
 
 // Element strides of a cache or of packed tokens (the last dimension is dense).
 struct Strides3 {

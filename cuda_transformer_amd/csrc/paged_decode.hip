@@ -80,56 +80,6 @@ template <int TILE>
 __device__ __forceinline__ int tiles_of(const PagedPlan& plan, int b) {
   return (plan.keys_to((int64_t)plan.lens[b] - 1) + TILE - 1) / TILE;
 }
-// Sum of the lanes' values below this lane, and (all) of the wave.
-__device__ __forceinline__ int64_t wave_scan(int64_t v, int64_t& all) {
-  const int lane = threadIdx.x & 63;
-  int64_t s = v;
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const int64_t o = __shfl_up(s, off);
-    if (lane >= off) s += o;
-  }
-  all = __shfl(s, 63);
-  return s - v;
-}
-// Tiles of all sequences (one job each); before: those of the sequences in front of b.
-template <int TILE>
-__device__ __forceinline__ int64_t count_tiles(const PagedPlan& plan, int b, int64_t& before) {
-  const int lane = threadIdx.x & 63;
-  int64_t total = 0, front = 0;
-  for (int i = lane; i - lane < plan.B; i += 64) {
-    const int64_t n = i < plan.B ? tiles_of<TILE>(plan, i) : 0;
-    total += n;
-    if (i < b) front += n;
-  }
-#pragma unroll
-  for (int off = 32; off >= 1; off >>= 1) {
-    total += __shfl_xor(total, off);
-    front += __shfl_xor(front, off);
-  }
-  before = front;
-  return total;
-}
-// Sequence that holds tile x of the sequences' tiles in a row (x < their number); before as above.
-template <int TILE>
-__device__ __forceinline__ int find_tile(const PagedPlan& plan, int64_t x, int64_t& before) {
-  const int lane = threadIdx.x & 63;
-  int64_t base = 0;
-  for (int i = lane; i - lane < plan.B; i += 64) {
-    const int64_t n = i < plan.B ? tiles_of<TILE>(plan, i) : 0;
-    int64_t all;
-    const int64_t at = base + wave_scan(n, all);
-    const uint64_t hit = __ballot(x >= at && x < at + n);
-    if (hit) {
-      const int w = __ffsll((unsigned long long)hit) - 1;
-      before = __shfl(at, w);
-      return i - lane + w;
-    }
-    base += all;
-  }
-  before = base;
-  return plan.B;
-}
 // First unit of workgroup w of W <= units: each has at least one.
 __device__ __forceinline__ int64_t deal_start(int64_t units, int w, int W) { return units * w / W; }
 
@@ -158,12 +108,13 @@ __global__ __launch_bounds__(256, 2) void paged_decode_kernel(DecodeArgs<E> a, P
     u_end = n_tiles;
   } else {
     int64_t before;
-    const int64_t units = count_tiles<TILE>(plan, 0, before) * jobs;
+    auto tiles = [&](int i) { return tiles_of<TILE>(plan, i); };
+    const int64_t units = count_tiles(plan.B, 0, before, tiles) * jobs;
     const int W = (int)min(units, (int64_t)gridDim.x);
     if ((int)blockIdx.x >= W) return;
     u = deal_start(units, blockIdx.x, W);
     u_end = deal_start(units, blockIdx.x + 1, W);
-    b = find_tile<TILE>(plan, u / jobs, before);
+    b = find_tile(plan.B, u / jobs, before, tiles);
     n_tiles = tiles_of<TILE>(plan, b);
     const int64_t in_seq = u - before * jobs;
     job = (int)(in_seq / n_tiles);
@@ -477,7 +428,8 @@ __global__ __launch_bounds__(256) void paged_decode_join_kernel(DecodeArgs<E> a,
   const int job = kvh * a.chunks + in_group / 16, row = in_group % 16;
   const int jobs = a.nkv * a.chunks;
   int64_t before;
-  const int64_t units = count_tiles<D::TILE>(plan, b, before) * jobs;
+  const int64_t units =
+      count_tiles(plan.B, b, before, [&](int i) { return tiles_of<D::TILE>(plan, i); }) * jobs;
   const int n = tiles_of<D::TILE>(plan, b);
   const int64_t at = (int64_t)b * a.nh + h;
   const int d = threadIdx.x % HS, pg = threadIdx.x / HS;

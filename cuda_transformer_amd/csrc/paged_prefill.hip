@@ -8,14 +8,18 @@
 //    workgroup has 128 rows (4 waves x 32) and walks their keys in stages, global -> registers ->
 //    LDS, double buffered, one barrier a stage.
 //  * Pages may end anywhere: for each stage 128 threads look the rows' addresses up two stages
-//    ahead and leave them in LDS, -1 for a row that holds no key.  Any page size takes this path.
+//    ahead and leave them in LDS, that of a row of zeros for a row that holds no key.  Any page
+//    size takes this path.
 //  * Both products are laid out as in the dense forward: S^T = K Q^T with a row's scores in one lane
 //    (lane l, register r: key R(r, l / 32) of row l % 32), so the maximum and sum of a row need one
-//    exchange, and P^T is the B operand of O^T += V^T P^T as it lies.  16-bit types: 32x32x16 MFMA, V
-//    transposed in LDS with bits 2 and 3 of the key swapped (kt_pos), probabilities rounded once to
-//    the type; FP32: 32x32x2 MFMA, V by rows.
-//  * Workgroups are ordered by head first (neighbours go to different XCDs, so an XCD's L2 holds few
-//    heads' keys), then from each sequence's last, longest tile to its first.
+//    exchange, and P^T is the B operand of O^T += V^T P^T as it lies.
+//  * 16-bit types: 32x32x16 MFMA, probabilities rounded once to the type.  K and V stages go straight
+//    from memory to LDS, by rows, and V's operand is read transposed (ds_read_b64_tr_b16: the 16
+//    lanes of a group read 16 d of 4 keys and get 4 keys of one d).  A row's 32-byte units are
+//    swapped by its number (row_swap), so that neither read of 8 rows meets a bank twice.
+//  * FP32: 32x32x2 MFMA, stages through registers.
+//  * Workgroups are ordered by head and split first (neighbours go to different XCDs, so an XCD's L2
+//    holds few heads' keys), then from each sequence's last, longest tile to its first.
 //  * Few rows on a long cache: `splits` workgroups share the stages of a tile and leave partial
 //    results in the workspace, which a second kernel joins in order.
 #include "paged.hpp"
@@ -43,270 +47,114 @@ __device__ __forceinline__ int tokens_of(const PagedPlan& plan, int N, int b, in
   return max(min(plan.cu_q[b + 1], N) - first, 0);
 }
 
+constexpr int BM = 128;              // rows a workgroup
+constexpr float kRescaleGap = 8.0f;  // log2 units: probabilities stay below 2^8
+
+// A workgroup's tile of rows: rows tile BM .. of the R that sequence b has for key/value head kvh.
+struct RowTile {
+  int b, first, R, tile, kvh, split;
+};
+// Finds it, or fills this workgroup's share of the padding rows and returns false.
 template <class E, int HS>
-__global__ __launch_bounds__(256, 2) void paged_prefill_kernel(PrefillArgs<E> a, PagedPlan plan) {
-  constexpr bool F32 = sizeof(E) == 4;
-  constexpr float kRescaleGap = 8.0f;  // log2 units: probabilities stay below 2^8
-  constexpr int BM = 128;              // rows
-  constexpr int BN = F32 ? 32 : 64;    // keys a stage
-  constexpr int V16 = 16 / sizeof(E);  // elements of 16 bytes
-  constexpr int KP = HS + V16;         // pitch of a K row
-  constexpr int VP = F32 ? HS + 8 : BN + 8;  // pitch of a V row, or of a V^T row (16-bit)
-  constexpr int KTILE = BN * KP, VTILE = F32 ? BN * VP : HS * VP;
-  constexpr int CH = HS / V16;         // 16-byte chunks a row
-  constexpr int LOADS = BN * CH / 256;
-  constexpr int VPAIRS = 32 * CH;      // row pairs of V chunks (16-bit)
-  constexpr int VL = F32 ? LOADS : 2 * ((VPAIRS + 255) / 256);
-  static_assert(LOADS >= 1 && BN * CH % 256 == 0, "a stage splits evenly over the threads");
-  __shared__ __attribute__((aligned(16))) E smem[2 * (KTILE + VTILE)];
-  __shared__ int64_t offs[2][2][BN];   // element offsets of a stage's K and V rows, -1: no key
-
-  const int tid = threadIdx.x, lane = tid & 63, wave = wave_index();
-  const int half = lane >> 5, col = lane & 31;
-  const int G = (int)a.group.d;
-  const int kvh = blockIdx.x % a.nkv, rest = blockIdx.x / a.nkv;
-  const int split = rest / a.tiles, x = rest - split * a.tiles;
-
+__device__ __forceinline__ bool find_rows(const PrefillArgs<E>& a, const PagedPlan& plan, RowTile& w) {
+  const int G = (int)a.group.d, tid = threadIdx.x;
+  const int x = blockIdx.x / (a.nkv * a.splits), rest = blockIdx.x - x * (a.nkv * a.splits);
+  w.split = rest / a.nkv;
+  w.kvh = rest - w.split * a.nkv;
   auto tiles_of = [&](int i) {
     int first;
     return ((int64_t)tokens_of(plan, a.N, i, first) * G + BM - 1) / BM;
   };
   int64_t before;
-  const int b = find_tile(plan.B, x, before, tiles_of);
-  if (b == plan.B) {  // no tile: rows of no sequence count as empty (the join writes them if split)
-    if (a.splits > 1) return;
-    const int spare = a.tiles - (int)min(before, (int64_t)a.tiles - 1);
-    const int lo = min(max(plan.cu_q[0], 0), a.N), hi = min(max(plan.cu_q[plan.B], lo), a.N);
-    const int64_t n = (int64_t)(a.N - (hi - lo)) * G;  // padding tokens x heads
-    for (int64_t i = x - before; i < n; i += spare) {
-      const int j = (int)(i / G), t = j < lo ? j : j - lo + hi;
-      const int64_t row = (int64_t)t * a.nh + kvh * G + (i - (int64_t)j * G);
-      if (tid < HS) a.o[row * HS + tid] = (E)0.0f;
-      if (tid == 0) a.l[row] = -INFINITY;
-    }
-    return;
+  w.b = find_tile(plan.B, x, before, tiles_of);
+  if (w.b < plan.B) {
+    w.R = tokens_of(plan, a.N, w.b, w.first) * G;
+    w.tile = (int)(tiles_of(w.b) - 1 - (x - before));
+    return true;
   }
-  int first;
-  const int R = tokens_of(plan, a.N, b, first) * G;
-  const int tile = (int)(tiles_of(b) - 1 - (x - before));
-  auto keys_at = [&](int r) {  // keys that row r sees
-    return plan.keys_to(plan.position(b, first + a.group.div(min(r, R - 1))));
-  };
-  const int r0 = tile * BM + wave * 32, my_r = r0 + col;
-  const bool live = my_r < R;
-  const int my_tok = first + a.group.div(min(my_r, R - 1));
-  const int my_head = kvh * G + min(my_r, R - 1) - (my_tok - first) * G;
-  const int my_keys = plan.keys_to(plan.position(b, my_tok));
-  const int wave_lo = keys_at(r0), wave_hi = r0 < R ? keys_at(r0 + 31) : 0;
-  const int n_keys = keys_at(tile * BM + BM - 1);
-  const int n_all = (n_keys + BN - 1) / BN;
-  const int s_begin = (int)((int64_t)n_all * split / a.splits);
-  const int s_end = (int)((int64_t)n_all * (split + 1) / a.splits);
-
-  // This lane's query row: the chunks of d that its half takes of each MFMA step
-  constexpr int QC = HS / (2 * V16);
-  u32x4 qf[QC];
-  {
-    const E* qp = a.q + my_tok * a.qt + my_head * a.qh + V16 * half;
-#pragma unroll
-    for (int s = 0; s < QC; ++s) qf[s] = *reinterpret_cast<const u32x4*>(qp + 2 * V16 * s);
+  // no tile: rows of no sequence count as empty (the join writes them if split)
+  if (a.splits > 1) return false;
+  const int spare = a.tiles - (int)min(before, (int64_t)a.tiles - 1);
+  const int lo = min(max(plan.cu_q[0], 0), a.N), hi = min(max(plan.cu_q[plan.B], lo), a.N);
+  const int64_t n = (int64_t)(a.N - (hi - lo)) * G;  // padding tokens x heads
+  for (int64_t i = x - before; i < n; i += spare) {
+    const int j = (int)(i / G), t = j < lo ? j : j - lo + hi;
+    const int64_t row = (int64_t)t * a.nh + w.kvh * G + (i - (int64_t)j * G);
+    if (tid < HS) a.o[row * HS + tid] = (E)0.0f;
+    if (tid == 0) a.l[row] = -INFINITY;
   }
+  return false;
+}
 
-  f32x16 oacc[HS / 32];
-#pragma unroll
-  for (int d = 0; d < HS / 32; ++d) oacc[d] = zero16();
-  float mb = -INFINITY, l_run = 0.0f;  // exponent offset, and this lane's part of the row's sum
+// The rows of one wave, one a lane (both halves): which they are and which keys they see.
+struct WaveRows {
+  bool live;
+  int token, head, keys;   // of this lane's row (the sequence's last one behind the end)
+  int lo, hi;              // the fewest and the most keys that a row of the wave sees
+  int n_keys;              // ... a row of the workgroup
+};
+template <class E>
+__device__ __forceinline__ WaveRows wave_rows(const PrefillArgs<E>& a, const PagedPlan& plan,
+                                              const RowTile& w, int wave, int col) {
+  auto token = [&](int r) { return w.first + a.group.div(min(r, w.R - 1)); };
+  auto keys = [&](int r) { return plan.keys_to(plan.position(w.b, token(r))); };
+  const int r0 = w.tile * BM + wave * 32, r = r0 + col;
+  WaveRows v;
+  v.live = r < w.R;
+  v.token = token(r);
+  v.head = w.kvh * (int)a.group.d + min(r, w.R - 1) - (v.token - w.first) * (int)a.group.d;
+  v.keys = keys(r);
+  v.lo = keys(r0);
+  v.hi = r0 < w.R ? keys(r0 + 31) : 0;
+  v.n_keys = keys(w.tile * BM + BM - 1);
+  return v;
+}
 
-  // Page of row `lane` of a stage, -1 for none: threads 0 .. BN - 1 for K, BN .. 2 BN - 1 for V.
-  const int32_t* table = plan.table + b * plan.table_stride;
-  auto look_up = [&](int stage) -> int64_t {
-    const int which = tid / BN, j = stage * BN + tid % BN;
-    if (which > 1 || stage >= s_end || j >= n_keys) return -1;
-    const int i = plan.ps.div(j), row = j - i * (int)plan.ps.d;
-    const int page = table[i];
-    if ((uint32_t)page >= (uint32_t)plan.num_pages) return -1;
-    return which == 0 ? page * a.sk.a + row * a.sk.r : page * a.sv.a + row * a.sv.r;
-  };
-  auto put = [&](int stage, int64_t off) {
-    if (tid < 2 * BN) offs[stage & 1][tid / BN][tid % BN] = off;
-  };
-
-  const E* kb = a.k + kvh * a.sk.h;
-  const E* vb = a.v + kvh * a.sv.h;
-  u32x4 kst[LOADS], vst[VL];
-  auto vtask = [&](int u2, int& rp, int& ch) {  // 16-bit: rows 2 rp, 2 rp + 1 of chunk ch
-    rp = lane & 31;
-    ch = 2 * (wave + 4 * u2) + (lane >> 5);
-    return VPAIRS % 256 == 0 || ch < CH;
-  };
-  // bit j: row j of the stage holds a key.  Rows that hold none read the first page's first row;
-  // their scores are masked, and their V counts as zeros.
-  auto gload = [&](int stage) -> uint64_t {
-    const int64_t(*of)[BN] = offs[stage & 1];
-    const uint64_t ok = __ballot(of[0][lane % BN] >= 0);
+// One online-softmax step: scaled scores s (N of this lane's row) become probabilities against the
+// row's offset mb, which moves only when some row of the wave sees a score more than kRescaleGap
+// above it; `rescale` scales the output.
+template <int N, class F>
+__device__ __forceinline__ void softmax_step(float (&s)[N], float& mb, float& l_run, F&& rescale) {
+  const float mb0 = mb == -INFINITY ? 0.0f : mb;
+  float t[N];
 #pragma unroll
-    for (int u = 0; u < LOADS; ++u) {
-      const int c = tid + 256 * u;
-      kst[u] = *reinterpret_cast<const u32x4*>(kb + max(of[0][c / CH], (int64_t)0) + V16 * (c % CH));
-    }
-    if constexpr (F32) {
-#pragma unroll
-      for (int u = 0; u < LOADS; ++u) {
-        const int c = tid + 256 * u;
-        const int64_t at = of[1][c / CH];
-        vst[u] = *reinterpret_cast<const u32x4*>(vb + max(at, (int64_t)0) + V16 * (c % CH));
-        if (at < 0) vst[u] = u32x4{0, 0, 0, 0};
-      }
-    } else {
-#pragma unroll
-      for (int u2 = 0; u2 < VL / 2; ++u2) {
-        int rp, ch;
-        if (!vtask(u2, rp, ch)) continue;
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int64_t at = of[1][2 * rp + e];
-          vst[2 * u2 + e] = *reinterpret_cast<const u32x4*>(vb + max(at, (int64_t)0) + V16 * ch);
-          if (at < 0) vst[2 * u2 + e] = u32x4{0, 0, 0, 0};
-        }
-      }
-    }
-    return ok;
-  };
-  auto lstore = [&](int buf) {
-    E* ks = smem + buf * (KTILE + VTILE);
-    E* vt = ks + KTILE;
-#pragma unroll
-    for (int u = 0; u < LOADS; ++u) {
-      const int c = tid + 256 * u;
-      *reinterpret_cast<u32x4*>(ks + (c / CH) * KP + V16 * (c % CH)) = kst[u];
-      if constexpr (F32)
-        *reinterpret_cast<u32x4*>(vt + (c / CH) * VP + V16 * (c % CH)) = vst[u];
-    }
-    if constexpr (!F32) {
-#pragma unroll
-      for (int u2 = 0; u2 < VL / 2; ++u2) {
-        int rp, ch;
-        if (!vtask(u2, rp, ch)) continue;
-        const u32x4 e0 = vst[2 * u2], e1 = vst[2 * u2 + 1];
-        uint32_t* col2 = reinterpret_cast<uint32_t*>(vt + kt_pos(2 * rp));
-#pragma unroll
-        for (int t = 0; t < 4; ++t) {  // d = 8 ch + 2 t and 8 ch + 2 t + 1 of both rows
-          col2[(8 * ch + 2 * t) * (VP / 2)] = pack_lo16(e0[t], e1[t]);
-          col2[(8 * ch + 2 * t + 1) * (VP / 2)] = pack_hi16(e0[t], e1[t]);
-        }
-      }
-    }
-  };
-
-  // Scaled scores of one 32-key tile -> probabilities against the row's offset, which moves only
-  // when some row of the wave sees a score more than kRescaleGap above it.
-  auto softmax_step = [&](f32x16& s) {
-    const float mb0 = mb == -INFINITY ? 0.0f : mb;
-    float t[16];
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      s[r] = __fsub_rn(s[r], mb0);
-      t[r] = s[r];
-    }
-    const float my = max_halves(max3_tree(t));
-    if (__any(mb == -INFINITY || my > kRescaleGap)) {
-      const float mb_new = fmaxf(mb, mb0 + my);
-      const float to = mb_new == -INFINITY ? 0.0f : mb_new;
-      const float alpha = fast_exp2(mb - to);
-      l_run *= alpha;
-#pragma unroll
-      for (int d = 0; d < HS / 32; ++d) oacc[d] *= alpha;
-      const float shift = to - mb0;
-#pragma unroll
-      for (int r = 0; r < 16; ++r) s[r] -= shift;
-      mb = mb_new;
-    }
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      s[r] = fast_exp2(s[r]);
-      t[r] = s[r];
-    }
-#pragma unroll
-    for (int w = 8; w >= 1; w >>= 1)
-#pragma unroll
-      for (int r = 0; r < w; ++r) t[r] += t[r + w];
-    l_run += t[0];
-  };
-
-  uint64_t mask = 0, mask_next = 0;
-  if (s_begin < s_end) {  // workgroup-uniform
-    put(s_begin, look_up(s_begin));
-    put(s_begin + 1, look_up(s_begin + 1));
-    __syncthreads();
-    mask = gload(s_begin);
-    lstore(s_begin & 1);
-    __syncthreads();
+  for (int r = 0; r < N; ++r) {
+    s[r] = __fsub_rn(s[r], mb0);
+    t[r] = s[r];
   }
-  for (int st = s_begin; st < s_end; ++st) {
-    const int64_t off2 = look_up(st + 2);
-    if (st + 1 < s_end) mask_next = gload(st + 1);
-    const E* ks = smem + (st & 1) * (KTILE + VTILE);
-    const E* vt = ks + KTILE;
+  const float my = max_halves(max3_tree(t));
+  if (__any(mb == -INFINITY || my > kRescaleGap)) {
+    const float mb_new = fmaxf(mb, mb0 + my);
+    const float to = mb_new == -INFINITY ? 0.0f : mb_new;
+    const float alpha = fast_exp2(mb - to);
+    l_run *= alpha;
+    rescale(alpha);
+    const float shift = to - mb0;
 #pragma unroll
-    for (int sub = 0; sub < BN / 32; ++sub) {
-      const int j0 = st * BN + 32 * sub;
-      if (j0 >= wave_hi) continue;  // no row of this wave sees the tile
-      const uint32_t ok = (uint32_t)(mask >> (32 * sub));
-      f32x16 s = zero16();
-      const E* krow = ks + (32 * sub + col) * KP + V16 * half;
-#pragma unroll
-      for (int c = 0; c < QC; ++c) {
-        const u32x4 kk = *reinterpret_cast<const u32x4*>(krow + 2 * V16 * c);
-        if constexpr (F32) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            s = mfma32(__uint_as_float(kk[i]), __uint_as_float(qf[c][i]), s);
-        } else {
-          s = Half16<E>::mfma(__builtin_bit_cast(vec8_t<E>, kk), __builtin_bit_cast(vec8_t<E>, qf[c]), s);
-        }
-      }
-      // rounded before the offset is taken off: equal scores of any size have equal exponents
-#pragma unroll
-      for (int r = 0; r < 16; ++r) s[r] = __fmul_rn(s[r], a.scale_log2);
-      if (j0 + 32 > wave_lo || ok != 0xffffffffu) {
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int j = mfma_row(r, half);
-          if (j0 + j >= my_keys || !(ok >> j & 1)) s[r] = -INFINITY;
-        }
-      }
-      softmax_step(s);
-      if constexpr (F32) {
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const E* vrow = vt + (32 * sub + mfma_row(r, half)) * VP + col;
-#pragma unroll
-          for (int d = 0; d < HS / 32; ++d) oacc[d] = mfma32(vrow[32 * d], s[r], oacc[d]);
-        }
-      } else {
-        vec8_t<E> pf[2];
-#pragma unroll
-        for (int r = 0; r < 16; ++r) pf[r >> 3][r & 7] = (E)s[r];
-#pragma unroll
-        for (int d = 0; d < HS / 32; ++d) {
-          const E* vrow = vt + (d * 32 + col) * VP + sub * 32 + 8 * half;
-#pragma unroll
-          for (int i = 0; i < 2; ++i)
-            oacc[d] = Half16<E>::mfma(ld8<E>(vrow + 16 * i), pf[i], oacc[d]);
-        }
-      }
-    }
-    mask = mask_next;
-    if (st + 1 < s_end) lstore((st + 1) & 1);
-    put(st + 2, off2);
-    __syncthreads();
+    for (int r = 0; r < N; ++r) s[r] -= shift;
+    mb = mb_new;
   }
+#pragma unroll
+  for (int r = 0; r < N; ++r) {
+    s[r] = fast_exp2(s[r]);
+    t[r] = s[r];
+  }
+#pragma unroll
+  for (int w = N / 2; w >= 1; w >>= 1)
+#pragma unroll
+    for (int r = 0; r < w; ++r) t[r] += t[r + w];
+  l_run += t[0];
+}
 
+// Writes a lane's part of its row: the result, or the split's part of it.
+template <class E, int HS>
+__device__ __forceinline__ void store_rows(const PrefillArgs<E>& a, const RowTile& w, const WaveRows& v,
+                                           const f32x16 (&oacc)[HS / 32], float mb, float l_run, int half) {
   const float l_tot = sum_halves(l_run);
-  if (!live) return;
-  const int64_t row = (int64_t)my_tok * a.nh + my_head;
+  if (!v.live) return;
+  const int64_t row = (int64_t)v.token * a.nh + v.head;
   if (a.splits > 1) {
-    const int64_t at = ((int64_t)split * a.N * a.nh) + row;
+    const int64_t at = (int64_t)w.split * a.N * a.nh + row;
     float* op = a.ws + at * HS;
 #pragma unroll
     for (int d = 0; d < HS / 32; ++d)
@@ -330,6 +178,281 @@ __global__ __launch_bounds__(256, 2) void paged_prefill_kernel(PrefillArgs<E> a,
       *reinterpret_cast<decltype(o4)*>(op + d * 32 + 8 * g + 4 * half) = o4;
     }
   if (half == 0) a.l[row] = l_tot == 0.0f ? -INFINITY : mb * kLn2 + logf(l_tot);
+}
+
+// What a row that holds no key reads.
+__device__ const float kZeroRow[128] = {};
+
+// Unit (32 bytes) of a row of RB bytes goes to unit ^ row_swap(row): eight consecutive rows spread
+// one unit over all 64 banks.
+template <int RB>
+__device__ __forceinline__ constexpr int row_swap(int row) {
+  return (row / (256 / RB)) & (RB / 32 - 1);
+}
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+// Four keys (rows) of this lane's d: lane i of a group of 16 reads 4 d of row i / 4 at p.
+__device__ __forceinline__ s16x4 ld_transposed(const void* p) {
+  return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p));
+}
+
+template <class E, int HS>
+__global__ __launch_bounds__(256, HS == 32 ? 3 : 2) void paged_prefill_half_kernel(PrefillArgs<E> a, PagedPlan plan) {
+  constexpr int BN = 64;           // keys a stage, one step of the softmax
+  constexpr int RB = 2 * HS;       // bytes of a row
+  constexpr int STAGE = BN * RB;   // bytes of K (or V) a stage
+  constexpr int COPIES = STAGE / 4096;      // 1 KiB copies a wave makes of each
+  constexpr int ROWS = 1024 / RB;  // rows a copy
+  constexpr int QC = HS / 16;      // MFMA steps of S over d
+  constexpr int ND = HS / 32;
+  // two buffers, apart so that reads of one are known not to meet the copies into the other
+  __shared__ __attribute__((aligned(16))) char buf0[2 * STAGE], buf1[2 * STAGE];
+  __shared__ uint64_t row_at[2][2][BN];  // addresses of a stage's K and V rows
+  __shared__ uint64_t holds[4];          // bit j: row j holds a key; four stages, as a slow wave
+                                         // may still look at a stage while the third is put
+
+  const int tid = threadIdx.x, lane = tid & 63, wave = wave_index();
+  const int half = lane >> 5, col = lane & 31;
+  RowTile w;
+  if (!find_rows<E, HS>(a, plan, w)) return;
+  const WaveRows v = wave_rows(a, plan, w, wave, col);
+  const int n_all = (v.n_keys + BN - 1) / BN;
+  const int s_begin = (int)((int64_t)n_all * w.split / a.splits);
+  const int s_end = (int)((int64_t)n_all * (w.split + 1) / a.splits);
+
+  // This lane's query row, d = 16 s + 8 half .. of step s
+  vec8_t<E> qf[QC];
+  {
+    const E* qp = a.q + v.token * a.qt + v.head * a.qh + 8 * half;
+#pragma unroll
+    for (int s = 0; s < QC; ++s) qf[s] = ld8<E>(qp + 16 * s);
+  }
+  f32x16 oacc[ND];
+#pragma unroll
+  for (int d = 0; d < ND; ++d) oacc[d] = zero16();
+  float mb = -INFINITY, l_run = 0.0f;  // exponent offset, and this lane's part of the row's sum
+
+  // Page of key `lane` of a stage, by waves 0 (K) and 1 (V); -1: none.
+  const int32_t* table = plan.table + w.b * plan.table_stride;
+  auto look_up = [&](int stage) {
+    const int j = stage * BN + lane;
+    return wave < 2 && stage < s_end && j < v.n_keys ? table[plan.ps.div(j)] : -1;
+  };
+  const E* kb = a.k + w.kvh * a.sk.h;
+  const E* vb = a.v + w.kvh * a.sv.h;
+  auto put = [&](int stage, int page) {
+    if (wave >= 2) return;
+    const int j = stage * BN + lane, row = j - plan.ps.div(j) * (int)plan.ps.d;
+    const bool ok = (uint32_t)page < (uint32_t)plan.num_pages;
+    const E* p = wave == 0 ? kb + page * a.sk.a + row * a.sk.r : vb + page * a.sv.a + row * a.sv.r;
+    row_at[stage & 1][wave][lane] = ok ? (uint64_t)p : (uint64_t)kZeroRow;
+    const uint64_t all = __ballot(ok);
+    if (tid == 0) holds[stage & 3] = all;
+  };
+  // Copy c of a stage: rows ROWS (4 c + wave) .., 16 bytes a lane, units swapped at the source.
+  const int c_row = ROWS * wave + lane / (RB / 16);
+  const int c_at = ((lane % (RB / 16) / 2) ^ row_swap<RB>(c_row)) * 32 + lane % 2 * 16;
+  auto copy = [&](int stage, char* to) {
+#pragma unroll
+    for (int kv = 0; kv < 2; ++kv)
+#pragma unroll
+      for (int c = 0; c < COPIES; ++c) {
+        const char* p = reinterpret_cast<const char*>(row_at[stage & 1][kv][4 * ROWS * c + c_row]) + c_at;
+        async_copy16(reinterpret_cast<const float*>(p),
+                     reinterpret_cast<float*>(to + kv * STAGE + 1024 * (4 * c + wave)));
+      }
+  };
+
+  // K operand: row col (+ 32), unit s of step s; V operand: rows 4 half + lane % 16 / 4 (+ 8 i),
+  // unit 2 d + lane / 16 % 2 of block d
+  int k_at[QC], v_at[ND];
+#pragma unroll
+  for (int s = 0; s < QC; ++s) k_at[s] = col * RB + (s ^ row_swap<RB>(col)) * 32 + 16 * half;
+  const int v_row = 4 * half + lane % 16 / 4;
+#pragma unroll
+  for (int d = 0; d < ND; ++d)
+    v_at[d] = v_row * RB + ((2 * d + lane / 16 % 2) ^ row_swap<RB>(v_row)) * 32 + lane % 4 * 8;
+
+  auto compute = [&](int st, const char* from) {
+    const int j0 = st * BN;
+    if (j0 >= v.hi) return;  // no row of this wave sees the stage
+    const uint64_t ok = holds[st & 3];
+    f32x16 s2[2] = {zero16(), zero16()};
+#pragma unroll
+    for (int c = 0; c < QC; ++c)
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        s2[i] = Half16<E>::mfma(*reinterpret_cast<const vec8_t<E>*>(from + k_at[c] + 32 * RB * i), qf[c], s2[i]);
+    // scaled and rounded before the offset is taken off: equal scores of any size have equal
+    // exponents
+    float s[32];
+#pragma unroll
+    for (int r = 0; r < 32; ++r) s[r] = __fmul_rn(s2[r >> 4][r & 15], a.scale_log2);
+    if (j0 + BN > v.lo || ~ok != 0) {
+#pragma unroll
+      for (int r = 0; r < 32; ++r) {
+        const int j = 32 * (r >> 4) + mfma_row(r & 15, half);
+        if (j0 + j >= v.keys || !(ok >> j & 1)) s[r] = -INFINITY;
+      }
+    }
+    softmax_step(s, mb, l_run, [&](float alpha) {
+#pragma unroll
+      for (int d = 0; d < ND; ++d) oacc[d] *= alpha;
+    });
+    vec8_t<E> pf[4];
+#pragma unroll
+    for (int r = 0; r < 32; ++r) pf[r >> 3][r & 7] = (E)s[r];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)  // 16 keys: the lane's 4 half + 0 .. 3 and 8 more
+#pragma unroll
+      for (int d = 0; d < ND; ++d) {
+        const char* p = from + STAGE + v_at[d] + 16 * RB * i;
+        struct { s16x4 a, b; } t = {ld_transposed(p), ld_transposed(p + 8 * RB)};
+        oacc[d] = Half16<E>::mfma(__builtin_bit_cast(vec8_t<E>, t), pf[i], oacc[d]);
+      }
+  };
+  auto step = [&](int st, const char* from, char* to) {
+    const int page = look_up(st + 2);
+    if (st + 1 < s_end) copy(st + 1, to);
+    compute(st, from);
+    put(st + 2, page);
+    vm_wait_all();
+    __syncthreads();
+  };
+
+  if (s_begin < s_end) {  // workgroup-uniform
+    put(s_begin, look_up(s_begin));
+    put(s_begin + 1, look_up(s_begin + 1));
+    __syncthreads();
+    copy(s_begin, buf0);
+    vm_wait_all();
+    __syncthreads();
+  }
+  for (int st = s_begin; st < s_end; st += 2) {
+    step(st, buf0, buf1);
+    if (st + 1 < s_end) step(st + 1, buf1, buf0);
+  }
+  store_rows<E, HS>(a, w, v, oacc, mb, l_run, half);
+}
+
+template <int HS>
+__global__ __launch_bounds__(256, 2) void paged_prefill_f32_kernel(PrefillArgs<float> a, PagedPlan plan) {
+  constexpr int BN = 32;            // keys a stage
+  constexpr int KP = HS + 4;        // pitch of a K row
+  constexpr int VP = HS + 8;        // pitch of a V row
+  constexpr int CH = HS / 4;        // 16-byte chunks a row
+  constexpr int LOADS = BN * CH / 256;
+  __shared__ __attribute__((aligned(16))) float smem[2][BN * (KP + VP)];
+  __shared__ uint64_t row_at[2][2][BN];  // addresses of a stage's K and V rows
+  __shared__ uint32_t holds[4];          // bit j: row j holds a key (four stages, as above)
+
+  const int tid = threadIdx.x, lane = tid & 63, wave = wave_index();
+  const int half = lane >> 5, col = lane & 31;
+  RowTile w;
+  if (!find_rows<float, HS>(a, plan, w)) return;
+  const WaveRows v = wave_rows(a, plan, w, wave, col);
+  const int n_all = (v.n_keys + BN - 1) / BN;
+  const int s_begin = (int)((int64_t)n_all * w.split / a.splits);
+  const int s_end = (int)((int64_t)n_all * (w.split + 1) / a.splits);
+
+  float4 qf[HS / 8];  // d = 8 s + 4 half ..
+  {
+    const float* qp = a.q + v.token * a.qt + v.head * a.qh + 4 * half;
+#pragma unroll
+    for (int s = 0; s < HS / 8; ++s) qf[s] = ld4(qp + 8 * s);
+  }
+  f32x16 oacc[HS / 32];
+#pragma unroll
+  for (int d = 0; d < HS / 32; ++d) oacc[d] = zero16();
+  float mb = -INFINITY, l_run = 0.0f;
+
+  // Page of a stage's key lane % 32, in wave 0: lanes 0 .. 31 for K, 32 .. 63 for V.
+  const int32_t* table = plan.table + w.b * plan.table_stride;
+  auto look_up = [&](int stage) {
+    const int j = stage * BN + col;
+    return wave == 0 && stage < s_end && j < v.n_keys ? table[plan.ps.div(j)] : -1;
+  };
+  const float* kb = a.k + w.kvh * a.sk.h;
+  const float* vb = a.v + w.kvh * a.sv.h;
+  auto put = [&](int stage, int page) {
+    if (wave != 0) return;
+    const int j = stage * BN + col, row = j - plan.ps.div(j) * (int)plan.ps.d;
+    const bool ok = (uint32_t)page < (uint32_t)plan.num_pages;
+    const float* p = half == 0 ? kb + page * a.sk.a + row * a.sk.r : vb + page * a.sv.a + row * a.sv.r;
+    row_at[stage & 1][half][col] = ok ? (uint64_t)p : (uint64_t)kZeroRow;
+    const uint64_t all = __ballot(ok);
+    if (tid == 0) holds[stage & 3] = (uint32_t)all;
+  };
+  float4 kst[LOADS], vst[LOADS];
+  auto gload = [&](int stage) {
+#pragma unroll
+    for (int u = 0; u < LOADS; ++u) {
+      const int c = tid + 256 * u;
+      kst[u] = ld4(reinterpret_cast<const float*>(row_at[stage & 1][0][c / CH]) + 4 * (c % CH));
+      vst[u] = ld4(reinterpret_cast<const float*>(row_at[stage & 1][1][c / CH]) + 4 * (c % CH));
+    }
+  };
+  auto lstore = [&](int stage) {
+    float* ks = smem[stage & 1];
+    float* vs = ks + BN * KP;
+#pragma unroll
+    for (int u = 0; u < LOADS; ++u) {
+      const int c = tid + 256 * u;
+      st4(ks + (c / CH) * KP + 4 * (c % CH), kst[u]);
+      st4(vs + (c / CH) * VP + 4 * (c % CH), vst[u]);
+    }
+  };
+  if (s_begin < s_end) {  // workgroup-uniform
+    put(s_begin, look_up(s_begin));
+    put(s_begin + 1, look_up(s_begin + 1));
+    __syncthreads();
+    gload(s_begin);
+    lstore(s_begin);
+    __syncthreads();
+  }
+  for (int st = s_begin; st < s_end; ++st) {
+    const int page = look_up(st + 2);
+    if (st + 1 < s_end) gload(st + 1);
+    const float* ks = smem[st & 1];
+    const float* vs = ks + BN * KP;
+    const int j0 = st * BN;
+    if (j0 < v.hi) {  // else no row of this wave sees the stage
+      const uint32_t ok = holds[st & 3];
+      f32x16 acc = zero16();
+#pragma unroll
+      for (int c = 0; c < HS / 8; ++c) {
+        const float4 k4 = ld4(ks + col * KP + 4 * half + 8 * c);
+        acc = mfma32(k4.x, qf[c].x, acc);
+        acc = mfma32(k4.y, qf[c].y, acc);
+        acc = mfma32(k4.z, qf[c].z, acc);
+        acc = mfma32(k4.w, qf[c].w, acc);
+      }
+      float s[16];
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] = __fmul_rn(acc[r], a.scale_log2);
+      if (j0 + BN > v.lo || ~ok != 0) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int j = mfma_row(r, half);
+          if (j0 + j >= v.keys || !(ok >> j & 1)) s[r] = -INFINITY;
+        }
+      }
+      softmax_step(s, mb, l_run, [&](float alpha) {
+#pragma unroll
+        for (int d = 0; d < HS / 32; ++d) oacc[d] *= alpha;
+      });
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+#pragma unroll
+        for (int d = 0; d < HS / 32; ++d)
+          oacc[d] = mfma32(vs[mfma_row(r, half) * VP + col + 32 * d], s[r], oacc[d]);
+    }
+    if (st + 1 < s_end) lstore(st + 1);
+    put(st + 2, page);
+    __syncthreads();
+  }
+  store_rows<float, HS>(a, w, v, oacc, mb, l_run, half);
 }
 
 // Joins the splits' parts of each row in order; padding rows.  A thread takes four elements.
@@ -374,15 +497,19 @@ struct PrefillGrid {
 PrefillGrid prefill_grid(int64_t B, int64_t N, int64_t nh, int64_t nkv, int64_t capacity) {
   PrefillGrid g;
   g.tiles = N * (nh / nkv) / 128 + std::min(B, N) + 1;
-  const int64_t fill = 512 / (std::max<int64_t>(g.tiles - 1, 1) * nkv);
+  const int64_t about = std::max<int64_t>(1, (N * (nh / nkv) + 64 * std::min(B, N)) / 128);
+  const int64_t fill = 512 / (about * nkv);
   g.splits = (int)std::max<int64_t>(1, std::min<int64_t>({fill, capacity / 512, 16}));
   return g;
 }
 
 template <class E, int HS>
 void launch_prefill(const PrefillArgs<E>& a, const PagedPlan& plan, hipStream_t st) {
-  hipLaunchKernelGGL((paged_prefill_kernel<E, HS>), dim3((unsigned)((int64_t)a.tiles * a.nkv * a.splits)),
-                     dim3(256), 0, st, a, plan);
+  const dim3 grid((unsigned)((int64_t)a.tiles * a.nkv * a.splits));
+  if constexpr (sizeof(E) == 4)
+    hipLaunchKernelGGL((paged_prefill_f32_kernel<HS>), grid, dim3(256), 0, st, a, plan);
+  else
+    hipLaunchKernelGGL((paged_prefill_half_kernel<E, HS>), grid, dim3(256), 0, st, a, plan);
   if (a.splits > 1)
     hipLaunchKernelGGL((paged_prefill_join_kernel<E, HS>),
                        dim3((unsigned)(((int64_t)a.N * a.nh * (HS / 4) + 255) / 256)), dim3(256), 0,

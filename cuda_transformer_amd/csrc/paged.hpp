@@ -68,6 +68,12 @@ struct PagedPlan {
   }
 };
 
+// A value that is the same in every lane, marked so: branches on it are scalar ones.
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ int64_t uniform(int64_t v) {
+  return (int64_t)((uint64_t)(uint32_t)uniform((int)(v >> 32)) << 32 | (uint32_t)uniform((int)v));
+}
+
 // Work counted in tiles, tiles(b) for sequence b: the host does not know the lengths, so a kernel
 // that shares it out counts them itself, 64 sequences a step.
 //
@@ -86,8 +92,8 @@ __device__ __forceinline__ int64_t count_tiles(int B, int b, int64_t& before, F&
     total += __shfl_xor(total, off);
     front += __shfl_xor(front, off);
   }
-  before = front;
-  return total;
+  before = uniform(front);
+  return uniform(total);
 }
 // Sequence that holds tile x of all tiles in a row, and the tiles before it; B, and all tiles, if
 // there are no more than x.  For a whole wave.
@@ -106,11 +112,11 @@ __device__ __forceinline__ int find_tile(int B, int64_t x, int64_t& before, F&& 
     }
     const uint64_t past = __ballot(before + end > x);
     if (past) {
-      const int w = __ffsll((unsigned long long)past) - 1;
-      before += __shfl(end - n, w);
+      const int w = __builtin_ctzll(past);
+      before += uniform(__shfl(end - n, w));
       return i0 + w;
     }
-    before += __shfl(end, 63);
+    before += uniform(__shfl(end, 63));
   }
   return B;
 }

@@ -15,8 +15,8 @@
 //    exchange, and P^T is the B operand of O^T += V^T P^T as it lies.
 //  * 16-bit types: 32x32x16 MFMA, probabilities rounded once to the type.  K and V stages go straight
 //    from memory to LDS, by rows, and V's operand is read transposed (ds_read_b64_tr_b16: the 16
-//    lanes of a group read 16 d of 4 keys and get 4 keys of one d).  A row's 32-byte units are
-//    swapped by its number (row_swap), so that neither read of 8 rows meets a bank twice.
+//    lanes of a group read 16 d of 4 keys and get 4 keys of one d).  A row's 16-byte chunks are
+//    swapped by its number (row_swap), so that neither read meets a bank twice.
 //  * FP32: 32x32x2 MFMA, stages through registers.
 //  * Workgroups are ordered by head and split first (neighbours go to different XCDs, so an XCD's L2
 //    holds few heads' keys), then from each sequence's last, longest tile to its first.
@@ -68,8 +68,10 @@ __device__ __forceinline__ bool find_rows(const PrefillArgs<E>& a, const PagedPl
   int64_t before;
   w.b = find_tile(plan.B, x, before, tiles_of);
   if (w.b < plan.B) {
-    w.R = tokens_of(plan, a.N, w.b, w.first) * G;
-    w.tile = (int)(tiles_of(w.b) - 1 - (x - before));
+    int first;
+    w.R = uniform(tokens_of(plan, a.N, w.b, first)) * G;
+    w.first = uniform(first);
+    w.tile = (w.R + BM - 1) / BM - 1 - (int)(x - before);
     return true;
   }
   // no tile: rows of no sequence count as empty (the join writes them if split)
@@ -97,53 +99,62 @@ template <class E>
 __device__ __forceinline__ WaveRows wave_rows(const PrefillArgs<E>& a, const PagedPlan& plan,
                                               const RowTile& w, int wave, int col) {
   auto token = [&](int r) { return w.first + a.group.div(min(r, w.R - 1)); };
-  auto keys = [&](int r) { return plan.keys_to(plan.position(w.b, token(r))); };
+  const int64_t p0 = uniform(plan.position(w.b, 0));  // of packed token 0, were it the sequence's
+  auto keys = [&](int r) { return plan.keys_to(p0 + token(r)); };
   const int r0 = w.tile * BM + wave * 32, r = r0 + col;
   WaveRows v;
   v.live = r < w.R;
   v.token = token(r);
   v.head = w.kvh * (int)a.group.d + min(r, w.R - 1) - (v.token - w.first) * (int)a.group.d;
   v.keys = keys(r);
-  v.lo = keys(r0);
-  v.hi = r0 < w.R ? keys(r0 + 31) : 0;
-  v.n_keys = keys(w.tile * BM + BM - 1);
+  v.lo = uniform(keys(r0));
+  v.hi = r0 < w.R ? uniform(keys(r0 + 31)) : 0;
+  v.n_keys = uniform(keys(w.tile * BM + BM - 1));
   return v;
 }
 
-// One online-softmax step: scaled scores s (N of this lane's row) become probabilities against the
-// row's offset mb, which moves only when some row of the wave sees a score more than kRescaleGap
-// above it; `rescale` scales the output.
-template <int N, class F>
-__device__ __forceinline__ void softmax_step(float (&s)[N], float& mb, float& l_run, F&& rescale) {
+// The first half of an online-softmax step: scores s (N of this lane's row) become exponents against
+// the row's offset mb, which moves only when some row of the wave sees one more than kRescaleGap
+// above it; `mask` sets those that do not count to -inf, `rescale` scales the output and the sum.
+// The exponent of score x is x c - mb in one rounding while offsets are small.  Beyond 2^20, where
+// the offset's own rounding would show, x c is rounded first: equal scores of any size then have
+// equal exponents.
+template <int N, class M, class F>
+__device__ __forceinline__ void exponents(float (&s)[N], float c, float& mb, M&& mask, F&& rescale) {
   const float mb0 = mb == -INFINITY ? 0.0f : mb;
+  if (__all(fabsf(mb0) <= 0x1p20f)) {
+#pragma unroll
+    for (int r = 0; r < N; ++r) s[r] = fmaf(s[r], c, -mb0);
+  } else {
+#pragma unroll
+    for (int r = 0; r < N; ++r) s[r] = __fsub_rn(__fmul_rn(s[r], c), mb0);
+  }
+  mask();
   float t[N];
 #pragma unroll
-  for (int r = 0; r < N; ++r) {
-    s[r] = __fsub_rn(s[r], mb0);
-    t[r] = s[r];
-  }
+  for (int r = 0; r < N; ++r) t[r] = s[r];
   const float my = max_halves(max3_tree(t));
   if (__any(mb == -INFINITY || my > kRescaleGap)) {
     const float mb_new = fmaxf(mb, mb0 + my);
     const float to = mb_new == -INFINITY ? 0.0f : mb_new;
-    const float alpha = fast_exp2(mb - to);
-    l_run *= alpha;
-    rescale(alpha);
+    rescale(fast_exp2(mb - to));
     const float shift = to - mb0;
 #pragma unroll
     for (int r = 0; r < N; ++r) s[r] -= shift;
     mb = mb_new;
   }
+}
+// 2^s in place, and their sum.
+template <int N>
+__device__ __forceinline__ float exp2_sum(float* s) {
+  float t[N];
 #pragma unroll
-  for (int r = 0; r < N; ++r) {
-    s[r] = fast_exp2(s[r]);
-    t[r] = s[r];
-  }
+  for (int r = 0; r < N; ++r) t[r] = s[r] = fast_exp2(s[r]);
 #pragma unroll
   for (int w = N / 2; w >= 1; w >>= 1)
 #pragma unroll
     for (int r = 0; r < w; ++r) t[r] += t[r + w];
-  l_run += t[0];
+  return t[0];
 }
 
 // Writes a lane's part of its row: the result, or the split's part of it.
@@ -183,11 +194,14 @@ __device__ __forceinline__ void store_rows(const PrefillArgs<E>& a, const RowTil
 // What a row that holds no key reads.
 __device__ const float kZeroRow[128] = {};
 
-// Unit (32 bytes) of a row of RB bytes goes to unit ^ row_swap(row): eight consecutive rows spread
-// one unit over all 64 banks.
+// Chunk c (16 bytes) of a row of RB bytes goes to chunk c ^ row_swap(row).  LDS serves 256 bytes a
+// cycle from 64 banks: 16 lanes of a 16-byte read (one chunk of 16 rows: the swap takes each value
+// of the chunks that share a row's banks once), 32 lanes of an 8-byte one (four chunks of 4 rows: the
+// swap's upper bits are those of the row that do not choose the bank yet).
 template <int RB>
 __device__ __forceinline__ constexpr int row_swap(int row) {
-  return (row / (256 / RB)) & (RB / 32 - 1);
+  const int low = row >> 2 & 3;
+  return RB == 256 ? (row & 3) << 2 | low : RB == 128 ? (row >> 1 & 1) << 2 | low : low;
 }
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
@@ -206,6 +220,8 @@ __global__ __launch_bounds__(256, HS == 32 ? 3 : 2) void paged_prefill_half_kern
   constexpr int ROWS = 1024 / RB;  // rows a copy
   constexpr int QC = HS / 16;      // MFMA steps of S over d
   constexpr int ND = HS / 32;
+  constexpr int kAhead = QC < 3 ? 2 * QC : 6;
+  constexpr int kDsRead = 0x100, kMfma = 0x8;  // instruction classes of sched_group_barrier
   // two buffers, apart so that reads of one are known not to meet the copies into the other
   __shared__ __attribute__((aligned(16))) char buf0[2 * STAGE], buf1[2 * STAGE];
   __shared__ uint64_t row_at[2][2][BN];  // addresses of a stage's K and V rows
@@ -250,9 +266,9 @@ __global__ __launch_bounds__(256, HS == 32 ? 3 : 2) void paged_prefill_half_kern
     const uint64_t all = __ballot(ok);
     if (tid == 0) holds[stage & 3] = all;
   };
-  // Copy c of a stage: rows ROWS (4 c + wave) .., 16 bytes a lane, units swapped at the source.
+  // Copy c of a stage: rows ROWS (4 c + wave) .., 16 bytes a lane, chunks swapped at the source.
   const int c_row = ROWS * wave + lane / (RB / 16);
-  const int c_at = ((lane % (RB / 16) / 2) ^ row_swap<RB>(c_row)) * 32 + lane % 2 * 16;
+  const int c_at = ((lane % (RB / 16)) ^ row_swap<RB>(c_row)) * 16;
   auto copy = [&](int stage, char* to) {
 #pragma unroll
     for (int kv = 0; kv < 2; ++kv)
@@ -264,15 +280,19 @@ __global__ __launch_bounds__(256, HS == 32 ? 3 : 2) void paged_prefill_half_kern
       }
   };
 
-  // K operand: row col (+ 32), unit s of step s; V operand: rows 4 half + lane % 16 / 4 (+ 8 i),
-  // unit 2 d + lane / 16 % 2 of block d
-  int k_at[QC], v_at[ND];
+  // K operand: row col (+ 32), chunk 2 s + half of step s.  V operand: rows 4 half + lane % 16 / 4
+  // (+ 16 i), 4 d from 32 d + 16 (lane / 16 % 2) + 4 (lane % 4) on; then 8 rows on, where the swap
+  // differs by 2 chunks.
+  int k_at[QC], v_at[2][ND];
 #pragma unroll
-  for (int s = 0; s < QC; ++s) k_at[s] = col * RB + (s ^ row_swap<RB>(col)) * 32 + 16 * half;
+  for (int s = 0; s < QC; ++s) k_at[s] = col * RB + ((2 * s + half) ^ row_swap<RB>(col)) * 16;
   const int v_row = 4 * half + lane % 16 / 4;
 #pragma unroll
-  for (int d = 0; d < ND; ++d)
-    v_at[d] = v_row * RB + ((2 * d + lane / 16 % 2) ^ row_swap<RB>(v_row)) * 32 + lane % 4 * 8;
+  for (int d = 0; d < ND; ++d) {
+    const int chunk = 4 * d + 2 * (lane / 16 % 2) + lane % 4 / 2;
+    v_at[0][d] = v_row * RB + (chunk ^ row_swap<RB>(v_row)) * 16 + lane % 2 * 8;
+    v_at[1][d] = v_at[0][d] ^ 32;
+  }
 
   auto compute = [&](int st, const char* from) {
     const int j0 = st * BN;
@@ -284,33 +304,45 @@ __global__ __launch_bounds__(256, HS == 32 ? 3 : 2) void paged_prefill_half_kern
 #pragma unroll
       for (int i = 0; i < 2; ++i)
         s2[i] = Half16<E>::mfma(*reinterpret_cast<const vec8_t<E>*>(from + k_at[c] + 32 * RB * i), qf[c], s2[i]);
-    // scaled and rounded before the offset is taken off: equal scores of any size have equal
-    // exponents
+    // the reads run ahead of the products by up to kAhead operands (LDS answers after about 100
+    // cycles, a product takes 32)
+    __builtin_amdgcn_sched_group_barrier(kDsRead, kAhead, 0);
+#pragma unroll
+    for (int i = 0; i < 2 * QC; ++i) {
+      __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
+      if (i + kAhead < 2 * QC) __builtin_amdgcn_sched_group_barrier(kDsRead, 1, 0);
+    }
     float s[32];
 #pragma unroll
-    for (int r = 0; r < 32; ++r) s[r] = __fmul_rn(s2[r >> 4][r & 15], a.scale_log2);
-    if (j0 + BN > v.lo || ~ok != 0) {
+    for (int r = 0; r < 32; ++r) s[r] = s2[r >> 4][r & 15];
+    exponents(
+        s, a.scale_log2, mb,
+        [&] {
+          if (j0 + BN <= v.lo && ~ok == 0) return;
 #pragma unroll
-      for (int r = 0; r < 32; ++r) {
-        const int j = 32 * (r >> 4) + mfma_row(r & 15, half);
-        if (j0 + j >= v.keys || !(ok >> j & 1)) s[r] = -INFINITY;
-      }
-    }
-    softmax_step(s, mb, l_run, [&](float alpha) {
+          for (int r = 0; r < 32; ++r) {
+            const int j = 32 * (r >> 4) + mfma_row(r & 15, half);
+            if (j0 + j >= v.keys || !(ok >> j & 1)) s[r] = -INFINITY;
+          }
+        },
+        [&](float alpha) {
+          l_run *= alpha;
 #pragma unroll
-      for (int d = 0; d < ND; ++d) oacc[d] *= alpha;
-    });
-    vec8_t<E> pf[4];
+          for (int d = 0; d < ND; ++d) oacc[d] *= alpha;
+        });
 #pragma unroll
-    for (int r = 0; r < 32; ++r) pf[r >> 3][r & 7] = (E)s[r];
+    for (int i = 0; i < 4; ++i) {  // 16 keys: the lane's 4 half + 0 .. 3 and 8 more
+      l_run += exp2_sum<8>(s + 8 * i);
+      vec8_t<E> pf;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)  // 16 keys: the lane's 4 half + 0 .. 3 and 8 more
+      for (int r = 0; r < 8; ++r) pf[r] = (E)s[8 * i + r];
 #pragma unroll
       for (int d = 0; d < ND; ++d) {
-        const char* p = from + STAGE + v_at[d] + 16 * RB * i;
-        struct { s16x4 a, b; } t = {ld_transposed(p), ld_transposed(p + 8 * RB)};
-        oacc[d] = Half16<E>::mfma(__builtin_bit_cast(vec8_t<E>, t), pf[i], oacc[d]);
+        const char* p = from + STAGE + 16 * RB * i;
+        struct { s16x4 a, b; } t = {ld_transposed(p + v_at[0][d]), ld_transposed(p + v_at[1][d] + 8 * RB)};
+        oacc[d] = Half16<E>::mfma(__builtin_bit_cast(vec8_t<E>, t), pf, oacc[d]);
       }
+    }
   };
   auto step = [&](int st, const char* from, char* to) {
     const int page = look_up(st + 2);
@@ -430,18 +462,23 @@ __global__ __launch_bounds__(256, 2) void paged_prefill_f32_kernel(PrefillArgs<f
       }
       float s[16];
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s[r] = __fmul_rn(acc[r], a.scale_log2);
-      if (j0 + BN > v.lo || ~ok != 0) {
+      for (int r = 0; r < 16; ++r) s[r] = acc[r];
+      exponents(
+          s, a.scale_log2, mb,
+          [&] {
+            if (j0 + BN <= v.lo && ~ok == 0) return;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int j = mfma_row(r, half);
-          if (j0 + j >= v.keys || !(ok >> j & 1)) s[r] = -INFINITY;
-        }
-      }
-      softmax_step(s, mb, l_run, [&](float alpha) {
+            for (int r = 0; r < 16; ++r) {
+              const int j = mfma_row(r, half);
+              if (j0 + j >= v.keys || !(ok >> j & 1)) s[r] = -INFINITY;
+            }
+          },
+          [&](float alpha) {
+            l_run *= alpha;
 #pragma unroll
-        for (int d = 0; d < HS / 32; ++d) oacc[d] *= alpha;
-      });
+            for (int d = 0; d < HS / 32; ++d) oacc[d] *= alpha;
+          });
+      l_run += exp2_sum<16>(s);
 #pragma unroll
       for (int r = 0; r < 16; ++r)
 #pragma unroll

@@ -275,6 +275,9 @@ __global__ __launch_bounds__(256, 2) void paged_decode_kernel(DecodeArgs<E> a, P
       load_v(t);
     }
     for (int tile = t; tile < t_end; ++tile) {
+      // no contraction: scaled scores are rounded before the offset is taken off, so that equal
+      // scores of any size have equal exponents
+#pragma clang fp contract(off)
       // ---- scores of 16 KG keys: lane, register r of group g: key 16 g + 4 quarter + r, head col
       f32x4 s[KG];
 #pragma unroll

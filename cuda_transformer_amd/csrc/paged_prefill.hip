@@ -17,12 +17,14 @@
 //    from memory to LDS, by rows, and V's operand is read transposed (ds_read_b64_tr_b16: the 16
 //    lanes of a group read 16 d of 4 keys and get 4 keys of one d).  A row's 16-byte chunks are
 //    swapped by its number (row_swap), so that neither read meets a bank twice.
-//  * FP32: 32x32x2 MFMA, stages through registers.
-//  * Workgroups are ordered by head and split first (neighbours go to different XCDs, so an XCD's L2
-//    holds few heads' keys), then from each sequence's last, longest tile to its first.
-//  * Few rows on a long cache: `splits` workgroups share the stages of a tile and leave partial
-//    results in the workspace, which a second kernel joins in order.
+//  * FP32: six BF16 products for one FP32 product, stages split on their way through registers.
+//  * Tiles differ in cost by any factor.  Many tiles: a workgroup each, heads side by side
+//    (neighbours go to different XCDs, so an XCD's L2 holds few heads' keys), each sequence's last,
+//    longest tile first.  Fewer: their cost is dealt evenly to as many workgroups as the GPU holds
+//    at once; the parts of a tile that several of them share go to the workspace, which a second
+//    kernel joins in order.  Both kernels compute the deal from cu_q and seq_lens.
 #include "paged.hpp"
+#include "split_bf16.hpp"
 
 namespace cta {
 namespace {
@@ -35,10 +37,12 @@ struct PrefillArgs {
   int N, nh, nkv;
   FastDiv group;
   float scale_log2;
-  int tiles, splits;  // tiles of 128 rows there may be; workgroups that share a tile's keys
+  int tiles;  // tiles of 128 rows that a key/value head may have
+  int W;      // workgroups that the tiles' cost is dealt to; 0: a workgroup a tile
+  int least;  // ... each of them at least this much
   E* o;
   float* l;
-  float* ws;          // splits > 1: O (splits, N nh, HS), then (m, l) (splits, N nh, 2)
+  float* ws;  // W > 0: O (2 W, 128, HS), then (m, l) (2 W, 128): a workgroup's first and last part
 };
 
 // Tokens of sequence b: first row and count, inside [0, N) whatever cu_q holds.
@@ -50,63 +54,202 @@ __device__ __forceinline__ int tokens_of(const PagedPlan& plan, int N, int b, in
 constexpr int BM = 128;              // rows a workgroup
 constexpr float kRescaleGap = 8.0f;  // log2 units: probabilities stay below 2^8
 
-// A workgroup's tile of rows: rows tile BM .. of the R that sequence b has for key/value head kvh.
+// What a workgroup works on: rows tile BM .. of the R that sequence b has for key/value head kvh,
+// and the share [lo, hi) of their `cost` units of work.
 struct RowTile {
-  int b, first, R, tile, kvh, split;
-};
-// Finds it, or fills this workgroup's share of the padding rows and returns false.
-template <class E, int HS>
-__device__ __forceinline__ bool find_rows(const PrefillArgs<E>& a, const PagedPlan& plan, RowTile& w) {
-  const int G = (int)a.group.d, tid = threadIdx.x;
-  const int x = blockIdx.x / (a.nkv * a.splits), rest = blockIdx.x - x * (a.nkv * a.splits);
-  w.split = rest / a.nkv;
-  w.kvh = rest - w.split * a.nkv;
-  auto tiles_of = [&](int i) {
-    int first;
-    return ((int64_t)tokens_of(plan, a.N, i, first) * G + BM - 1) / BM;
-  };
-  int64_t before;
-  w.b = find_tile(plan.B, x, before, tiles_of);
-  if (w.b < plan.B) {
-    int first;
-    w.R = uniform(tokens_of(plan, a.N, w.b, first)) * G;
-    w.first = uniform(first);
-    w.tile = (w.R + BM - 1) / BM - 1 - (int)(x - before);
-    return true;
+  int b, first, R, tile, kvh;
+  int64_t lo, hi, cost;
+  __device__ __forceinline__ bool whole() const { return lo == 0 && hi == cost; }
+  // The share of n stages.
+  __device__ __forceinline__ int stage(int64_t at, int n) const {
+    return at == 0 ? 0 : at == cost ? n : (int)(n * at / cost);
   }
-  // no tile: rows of no sequence count as empty (the join writes them if split)
-  if (a.splits > 1) return false;
-  const int spare = a.tiles - (int)min(before, (int64_t)a.tiles - 1);
+};
+// Work of a sequence's tiles: tile q costs past + 128 (q + 1), the keys that its last row would see
+// (times group) were the tile full.  Every cost is positive, and the sum of the first q has a
+// closed form.
+struct SeqCost {
+  int first, R;
+  int64_t past;
+  __device__ __forceinline__ int tiles() const { return (R + BM - 1) / BM; }
+  __device__ __forceinline__ int64_t upto(int64_t q) const { return q * past + BM / 2 * q * (q + 1); }
+};
+template <class E>
+__device__ __forceinline__ SeqCost seq_cost(const PrefillArgs<E>& a, const PagedPlan& plan, int b) {
+  SeqCost c;
+  c.R = tokens_of(plan, a.N, b, c.first) * (int)a.group.d;
+  c.past = (int64_t)plan.keys_to(plan.position(b, c.first) - 1) * a.group.d;
+  return c;
+}
+// Tile x of a head, all sequences' tiles in a row; false: there are fewer (then before is their
+// number).
+template <class E>
+__device__ __forceinline__ bool find_rows(const PrefillArgs<E>& a, const PagedPlan& plan, int x,
+                                          RowTile& w, int64_t& before) {
+  w.b = find_tile(plan.B, x, before, [&](int i) { return (int64_t)seq_cost(a, plan, i).tiles(); });
+  if (w.b == plan.B) return false;
+  const SeqCost c = seq_cost(a, plan, w.b);
+  w.first = uniform(c.first);
+  w.R = uniform(c.R);
+  w.tile = x - (int)before;
+  w.cost = uniform(c.past) + BM * (int64_t)(w.tile + 1);
+  w.lo = 0;
+  w.hi = w.cost;
+  return true;
+}
+// How the work of all heads' tiles, units in a row, is dealt to W workgroups: about units / W each.
+// A cut that would fall within `slack` of a tile's end is made there: small pieces cost more than
+// they balance.
+struct Deal {
+  int64_t head, units, slack;  // units of one head, of all of them
+  int W;
+  __device__ __forceinline__ int64_t cut(int n) const { return units * n / W; }
+  // The last workgroup whose cut is at or before u.
+  __device__ __forceinline__ int owner(int64_t u) const { return (int)(((u + 1) * W - 1) / units); }
+  // Distance from its ends within which a tile is not cut.
+  __device__ __forceinline__ int64_t edge(int64_t cost) const { return min(slack, cost / 4); }
+};
+template <class E>
+__device__ __forceinline__ Deal make_deal(const PrefillArgs<E>& a, const PagedPlan& plan, int b,
+                                          int64_t& before) {
+  Deal d;
+  d.head = count_tiles(plan.B, b, before, [&](int i) {
+    const SeqCost c = seq_cost(a, plan, i);
+    return c.upto(c.tiles());
+  });
+  d.units = d.head * a.nkv;
+  d.W = (int)max((int64_t)1, min((int64_t)a.W, d.units / a.least));
+  d.slack = d.units / d.W / 8;
+  return d;
+}
+// The tile that holds unit u, which is made relative to the tile's begin.
+template <class E>
+__device__ __forceinline__ void find_unit(const PrefillArgs<E>& a, const PagedPlan& plan,
+                                          const Deal& d, int64_t& u, RowTile& w) {
+  w.kvh = (int)(u / d.head);
+  u -= w.kvh * d.head;
+  int64_t before;
+  w.b = find_tile(plan.B, u, before, [&](int i) {
+    const SeqCost c = seq_cost(a, plan, i);
+    return c.upto(c.tiles());
+  });
+  SeqCost c = seq_cost(a, plan, w.b);
+  w.first = c.first = uniform(c.first);
+  w.R = c.R = uniform(c.R);
+  c.past = uniform(c.past);
+  u -= before;
+  int q = 0;  // the last tile that begins at or before u
+  for (int n = c.tiles(); n > 1;) {
+    const int h = n / 2;
+    if (c.upto(q + h) <= u) { q += h; n -= h; }
+    else n = h;
+  }
+  u -= c.upto(q);
+  w.tile = q;
+  w.cost = c.past + BM * (int64_t)(q + 1);
+}
+// The next tile of the deal (there is one).
+template <class E>
+__device__ __forceinline__ void next_tile(const PrefillArgs<E>& a, const PagedPlan& plan, RowTile& w) {
+  if ((w.tile + 1) * BM < w.R) {
+    ++w.tile;
+    w.cost += BM;
+    return;
+  }
+  SeqCost c;
+  do {
+    if (++w.b == plan.B) { w.b = 0; ++w.kvh; }
+    c = seq_cost(a, plan, w.b);
+    w.R = uniform(c.R);
+  } while (w.R == 0);
+  w.first = uniform(c.first);
+  w.tile = 0;
+  w.cost = uniform(c.past) + BM;
+}
+// Rows of no sequence count as empty: share i of n of them, for head kvh.
+template <class E, int HS>
+__device__ __forceinline__ void fill_padding(const PrefillArgs<E>& a, const PagedPlan& plan, int kvh,
+                                             int i, int n) {
+  const int G = (int)a.group.d, tid = threadIdx.x;
   const int lo = min(max(plan.cu_q[0], 0), a.N), hi = min(max(plan.cu_q[plan.B], lo), a.N);
-  const int64_t n = (int64_t)(a.N - (hi - lo)) * G;  // padding tokens x heads
-  for (int64_t i = x - before; i < n; i += spare) {
-    const int j = (int)(i / G), t = j < lo ? j : j - lo + hi;
-    const int64_t row = (int64_t)t * a.nh + w.kvh * G + (i - (int64_t)j * G);
+  const int64_t rows = (int64_t)(a.N - (hi - lo)) * G;  // padding tokens x heads
+  for (int64_t r = i; r < rows; r += n) {
+    const int j = (int)(r / G), t = j < lo ? j : j - lo + hi;
+    const int64_t row = (int64_t)t * a.nh + kvh * G + (r - (int64_t)j * G);
     if (tid < HS) a.o[row * HS + tid] = (E)0.0f;
     if (tid == 0) a.l[row] = -INFINITY;
   }
-  return false;
+}
+// Calls body(tile, slot of the workspace for a part of it) for each of this workgroup's tiles: one, or
+// (DEAL) those of its share.
+template <class E, int HS, bool DEAL, class F>
+__device__ __forceinline__ void each_tile(const PrefillArgs<E>& a, const PagedPlan& plan, F&& body) {
+  RowTile w;
+  int64_t before;
+  if constexpr (!DEAL) {
+    // longest first: x counts a sequence's tiles from the last
+    const int x = blockIdx.x / a.nkv;
+    w.kvh = blockIdx.x - x * a.nkv;
+    if (!find_rows(a, plan, x, w, before)) {
+      const int base = (int)min(before, (int64_t)a.tiles - 1);
+      fill_padding<E, HS>(a, plan, w.kvh, x - base, a.tiles - base);
+      return;
+    }
+    w.tile = (w.R + BM - 1) / BM - 1 - w.tile;
+    body(w, 0);
+  } else {
+    const Deal deal = make_deal(a, plan, 0, before);
+    const int n = xcd_work_item(blockIdx.x, deal.W);  // an XCD has neighbouring shares: few heads
+    if ((int)blockIdx.x / kNumXcds >= (deal.W + kNumXcds - 1) / kNumXcds) return;
+    if (n >= deal.W) return;
+    int64_t u = deal.cut(n);
+    int64_t left = deal.cut(n + 1) - u;  // units from the tile's begin to this workgroup's end
+    if (left == 0) return;
+    find_unit(a, plan, deal, u, w);
+    left += u;
+    w.lo = u <= deal.edge(w.cost) ? 0 : u;
+    if (u >= w.cost - deal.edge(w.cost)) {  // the share begins at the next tile
+      left -= w.cost;
+      w.lo = 0;
+      if (left <= 0) return;
+      next_tile(a, plan, w);
+    }
+    for (;;) {
+      const int64_t edge = deal.edge(w.cost);
+      if (w.lo == 0 && left <= edge) return;  // the tile is the next workgroup's
+      w.hi = left >= w.cost - edge ? w.cost : left;
+      // a tile that began in an earlier workgroup goes to this one's first slot, else to its second
+      body(w, 2 * n + (w.lo == 0));
+      left -= w.cost;
+      if (left <= 0) return;
+      w.lo = 0;
+      next_tile(a, plan, w);
+    }
+  }
 }
 
-// The rows of one wave, one a lane (both halves): which they are and which keys they see.
+// Token and query head of row r of a tile's sequence (its last row behind the end).
+template <class E>
+__device__ __forceinline__ void row_of(const PrefillArgs<E>& a, const RowTile& w, int r, int& token, int& head) {
+  r = min(r, w.R - 1);
+  const int i = a.group.div(r);
+  token = w.first + i;
+  head = w.kvh * (int)a.group.d + r - i * (int)a.group.d;
+}
+// Which keys the rows of one wave see, one row a lane (both halves).
 struct WaveRows {
-  bool live;
-  int token, head, keys;   // of this lane's row (the sequence's last one behind the end)
-  int lo, hi;              // the fewest and the most keys that a row of the wave sees
-  int n_keys;              // ... a row of the workgroup
+  int keys;    // this lane's row
+  int lo, hi;  // the fewest and the most of the wave's rows
+  int n_keys;  // the most of the workgroup's rows
 };
 template <class E>
 __device__ __forceinline__ WaveRows wave_rows(const PrefillArgs<E>& a, const PagedPlan& plan,
                                               const RowTile& w, int wave, int col) {
-  auto token = [&](int r) { return w.first + a.group.div(min(r, w.R - 1)); };
-  const int64_t p0 = uniform(plan.position(w.b, 0));  // of packed token 0, were it the sequence's
-  auto keys = [&](int r) { return plan.keys_to(p0 + token(r)); };
-  const int r0 = w.tile * BM + wave * 32, r = r0 + col;
+  const int64_t p0 = uniform(plan.position(w.b, w.first));
+  auto keys = [&](int r) { return plan.keys_to(p0 + a.group.div(min(r, w.R - 1))); };
+  const int r0 = w.tile * BM + wave * 32;
   WaveRows v;
-  v.live = r < w.R;
-  v.token = token(r);
-  v.head = w.kvh * (int)a.group.d + min(r, w.R - 1) - (v.token - w.first) * (int)a.group.d;
-  v.keys = keys(r);
+  v.keys = keys(r0 + col);
   v.lo = uniform(keys(r0));
   v.hi = r0 < w.R ? uniform(keys(r0 + 31)) : 0;
   v.n_keys = uniform(keys(w.tile * BM + BM - 1));
@@ -126,8 +269,12 @@ __device__ __forceinline__ void exponents(float (&s)[N], float c, float& mb, M&&
 #pragma unroll
     for (int r = 0; r < N; ++r) s[r] = fmaf(s[r], c, -mb0);
   } else {
+#pragma clang fp contract(off)
 #pragma unroll
-    for (int r = 0; r < N; ++r) s[r] = __fsub_rn(__fmul_rn(s[r], c), mb0);
+    for (int r = 0; r < N; ++r) {
+      const float x = s[r] * c;
+      s[r] = x - mb0;
+    }
   }
   mask();
   float t[N];
@@ -157,26 +304,31 @@ __device__ __forceinline__ float exp2_sum(float* s) {
   return t[0];
 }
 
-// Writes a lane's part of its row: the result, or the split's part of it.
+// Writes a lane's part of its row: the result, or the share's part of it (`any`: it had stages).
 template <class E, int HS>
-__device__ __forceinline__ void store_rows(const PrefillArgs<E>& a, const RowTile& w, const WaveRows& v,
-                                           const f32x16 (&oacc)[HS / 32], float mb, float l_run, int half) {
+__device__ __forceinline__ void store_rows(const PrefillArgs<E>& a, const RowTile& w, int slot,
+                                           const f32x16 (&oacc)[HS / 32], float mb, float l_run, bool any) {
+  const int lane = threadIdx.x & 63, half = lane >> 5, in_tile = wave_index() * 32 + (lane & 31);
   const float l_tot = sum_halves(l_run);
-  if (!v.live) return;
-  const int64_t row = (int64_t)v.token * a.nh + v.head;
-  if (a.splits > 1) {
-    const int64_t at = (int64_t)w.split * a.N * a.nh + row;
+  if (w.tile * BM + in_tile >= w.R) return;
+  if (!w.whole()) {
+    const int64_t at = (int64_t)slot * BM + in_tile;
     float* op = a.ws + at * HS;
+    if (any) {
 #pragma unroll
-    for (int d = 0; d < HS / 32; ++d)
+      for (int d = 0; d < HS / 32; ++d)
 #pragma unroll
-      for (int g = 0; g < 4; ++g)
-        st4(op + d * 32 + 8 * g + 4 * half, make_float4(oacc[d][4 * g], oacc[d][4 * g + 1],
-                                                        oacc[d][4 * g + 2], oacc[d][4 * g + 3]));
+        for (int g = 0; g < 4; ++g)
+          st4(op + d * 32 + 8 * g + 4 * half, make_float4(oacc[d][4 * g], oacc[d][4 * g + 1],
+                                                          oacc[d][4 * g + 2], oacc[d][4 * g + 3]));
+    }
     if (half == 0)
-      *reinterpret_cast<float2*>(a.ws + (int64_t)a.splits * a.N * a.nh * HS + at * 2) = make_float2(mb, l_tot);
+      *reinterpret_cast<float2*>(a.ws + (int64_t)2 * a.W * BM * HS + at * 2) = make_float2(mb, l_tot);
     return;
   }
+  int token, head;
+  row_of(a, w, w.tile * BM + in_tile, token, head);
+  const int64_t row = (int64_t)token * a.nh + head;
   E* op = a.o + row * HS;
   const float inv = l_tot == 0.0f ? 0.0f : 1.0f / l_tot;
 #pragma unroll
@@ -211,7 +363,7 @@ __device__ __forceinline__ s16x4 ld_transposed(const void* p) {
   return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p));
 }
 
-template <class E, int HS>
+template <class E, int HS, bool DEAL>
 __global__ __launch_bounds__(256, HS == 32 ? 3 : 2) void paged_prefill_half_kernel(PrefillArgs<E> a, PagedPlan plan) {
   constexpr int BN = 64;           // keys a stage, one step of the softmax
   constexpr int RB = 2 * HS;       // bytes of a row
@@ -230,17 +382,18 @@ __global__ __launch_bounds__(256, HS == 32 ? 3 : 2) void paged_prefill_half_kern
 
   const int tid = threadIdx.x, lane = tid & 63, wave = wave_index();
   const int half = lane >> 5, col = lane & 31;
-  RowTile w;
-  if (!find_rows<E, HS>(a, plan, w)) return;
+  each_tile<E, HS, DEAL>(a, plan, [&](const RowTile& w, int slot) {
   const WaveRows v = wave_rows(a, plan, w, wave, col);
   const int n_all = (v.n_keys + BN - 1) / BN;
-  const int s_begin = (int)((int64_t)n_all * w.split / a.splits);
-  const int s_end = (int)((int64_t)n_all * (w.split + 1) / a.splits);
+  const int s_begin = w.stage(w.lo, n_all);
+  const int s_end = w.stage(w.hi, n_all);
 
   // This lane's query row, d = 16 s + 8 half .. of step s
   vec8_t<E> qf[QC];
   {
-    const E* qp = a.q + v.token * a.qt + v.head * a.qh + 8 * half;
+    int token, head;
+    row_of(a, w, w.tile * BM + wave * 32 + col, token, head);
+    const E* qp = a.q + token * a.qt + head * a.qh + 8 * half;
 #pragma unroll
     for (int s = 0; s < QC; ++s) qf[s] = ld8<E>(qp + 16 * s);
   }
@@ -282,28 +435,25 @@ __global__ __launch_bounds__(256, HS == 32 ? 3 : 2) void paged_prefill_half_kern
 
   // K operand: row col (+ 32), chunk 2 s + half of step s.  V operand: rows 4 half + lane % 16 / 4
   // (+ 16 i), 4 d from 32 d + 16 (lane / 16 % 2) + 4 (lane % 4) on; then 8 rows on, where the swap
-  // differs by 2 chunks.
-  int k_at[QC], v_at[2][ND];
-#pragma unroll
-  for (int s = 0; s < QC; ++s) k_at[s] = col * RB + ((2 * s + half) ^ row_swap<RB>(col)) * 16;
+  // differs by 2 chunks.  Steps and blocks differ by the bits 32 s and 64 d of the address.
   const int v_row = 4 * half + lane % 16 / 4;
-#pragma unroll
-  for (int d = 0; d < ND; ++d) {
-    const int chunk = 4 * d + 2 * (lane / 16 % 2) + lane % 4 / 2;
-    v_at[0][d] = v_row * RB + (chunk ^ row_swap<RB>(v_row)) * 16 + lane % 2 * 8;
-    v_at[1][d] = v_at[0][d] ^ 32;
-  }
+  const int k_lane = col * RB + (half ^ row_swap<RB>(col)) * 16;
+  const int v_lane = v_row * RB + ((2 * (lane / 16 % 2) + lane % 4 / 2) ^ row_swap<RB>(v_row)) * 16 + lane % 2 * 8;
 
   auto compute = [&](int st, const char* from) {
     const int j0 = st * BN;
     if (j0 >= v.hi) return;  // no row of this wave sees the stage
     const uint64_t ok = holds[st & 3];
+    // made anew each stage: fourteen registers less to keep
+    int k_at = k_lane, v_at = v_lane;
+    asm volatile("" : "+v"(k_at), "+v"(v_at));
     f32x16 s2[2] = {zero16(), zero16()};
 #pragma unroll
     for (int c = 0; c < QC; ++c)
 #pragma unroll
       for (int i = 0; i < 2; ++i)
-        s2[i] = Half16<E>::mfma(*reinterpret_cast<const vec8_t<E>*>(from + k_at[c] + 32 * RB * i), qf[c], s2[i]);
+        s2[i] = Half16<E>::mfma(
+            *reinterpret_cast<const vec8_t<E>*>(from + (k_at ^ 32 * c) + 32 * RB * i), qf[c], s2[i]);
     // the reads run ahead of the products by up to kAhead operands (LDS answers after about 100
     // cycles, a product takes 32)
     __builtin_amdgcn_sched_group_barrier(kDsRead, kAhead, 0);
@@ -339,7 +489,8 @@ __global__ __launch_bounds__(256, HS == 32 ? 3 : 2) void paged_prefill_half_kern
 #pragma unroll
       for (int d = 0; d < ND; ++d) {
         const char* p = from + STAGE + 16 * RB * i;
-        struct { s16x4 a, b; } t = {ld_transposed(p + v_at[0][d]), ld_transposed(p + v_at[1][d] + 8 * RB)};
+        struct { s16x4 a, b; } t = {ld_transposed(p + (v_at ^ 64 * d)),
+                                    ld_transposed(p + (v_at ^ 64 * d ^ 32) + 8 * RB)};
         oacc[d] = Half16<E>::mfma(__builtin_bit_cast(vec8_t<E>, t), pf, oacc[d]);
       }
     }
@@ -365,38 +516,59 @@ __global__ __launch_bounds__(256, HS == 32 ? 3 : 2) void paged_prefill_half_kern
     step(st, buf0, buf1);
     if (st + 1 < s_end) step(st + 1, buf1, buf0);
   }
-  store_rows<E, HS>(a, w, v, oacc, mb, l_run, half);
+  store_rows<E, HS>(a, w, slot, oacc, mb, l_run, s_begin < s_end);
+  });
 }
 
-template <int HS>
-__global__ __launch_bounds__(256, 2) void paged_prefill_f32_kernel(PrefillArgs<float> a, PagedPlan plan) {
-  constexpr int BN = 32;            // keys a stage
-  constexpr int KP = HS + 4;        // pitch of a K row
-  constexpr int VP = HS + 8;        // pitch of a V row
-  constexpr int CH = HS / 4;        // 16-byte chunks a row
-  constexpr int LOADS = BN * CH / 256;
-  __shared__ __attribute__((aligned(16))) float smem[2][BN * (KP + VP)];
+// FP32.  Both products run as six BF16 products of three-part operands (split_bf16.hpp), laid out
+// and scaled as in the dense forward: Q, P and V by 2^24, sums of the first parts and of the smaller
+// ones apart.  A workgroup that meets a query beyond the parts' range, or whose sums are not finite,
+// walks its keys again on the FP32 MFMA.
+template <int HS, bool DEAL>
+__global__ __launch_bounds__(256, HS == 128 ? 1 : 2) void paged_prefill_f32_kernel(
+    PrefillArgs<float> a, PagedPlan plan) {
+  constexpr int BN = 32;               // keys a stage
+  constexpr int PART = BN * HS * 2;    // bytes of one part of a stage's K (or V)
+  constexpr int STAGE = 6 * PART;
+  constexpr int UNITS = BN * HS / 8;   // 16-byte units of a part
+  constexpr int NU = (UNITS + 255) / 256;
+  constexpr int KP = HS + 4, VP = HS + 8;  // row pitches of an FP32 stage
+  static_assert(BN * (KP + VP) * 4 <= 2 * STAGE, "an FP32 stage fits");
+  __shared__ __attribute__((aligned(16))) char smem[2 * STAGE];
   __shared__ uint64_t row_at[2][2][BN];  // addresses of a stage's K and V rows
   __shared__ uint32_t holds[4];          // bit j: row j holds a key (four stages, as above)
 
   const int tid = threadIdx.x, lane = tid & 63, wave = wave_index();
   const int half = lane >> 5, col = lane & 31;
-  RowTile w;
-  if (!find_rows<float, HS>(a, plan, w)) return;
+  each_tile<float, HS, DEAL>(a, plan, [&](const RowTile& w, int slot) {
   const WaveRows v = wave_rows(a, plan, w, wave, col);
   const int n_all = (v.n_keys + BN - 1) / BN;
-  const int s_begin = (int)((int64_t)n_all * w.split / a.splits);
-  const int s_end = (int)((int64_t)n_all * (w.split + 1) / a.splits);
+  const int s_begin = w.stage(w.lo, n_all);
+  const int s_end = w.stage(w.hi, n_all);
 
-  float4 qf[HS / 8];  // d = 8 s + 4 half ..
-  {
-    const float* qp = a.q + v.token * a.qt + v.head * a.qh + 4 * half;
+  // Parts of this lane's query row, d = 16 s + 8 half .. of step s
+  int token, head;
+  row_of(a, w, w.tile * BM + wave * 32 + col, token, head);
+  const float* qrow = a.q + token * a.qt + head * a.qh;
+  bf16x8 qp[HS / 16][3];
+  float qmax = 0.0f;
 #pragma unroll
-    for (int s = 0; s < HS / 8; ++s) qf[s] = ld4(qp + 8 * s);
+  for (int s = 0; s < HS / 16; ++s) {
+    float x[8];
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const float4 q4 = ld4(qrow + 16 * s + 8 * half + 4 * c);
+      x[4 * c] = q4.x; x[4 * c + 1] = q4.y; x[4 * c + 2] = q4.z; x[4 * c + 3] = q4.w;
+    }
+    split_bf16<true>(x, qp[s]);
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) qmax = fmaxf(fmaxf(qmax, fabsf(x[e])), fabsf(x[e + 1]));
   }
-  f32x16 oacc[HS / 32];
+  bool odd = __any(qmax >= kMaxScoreFactor);
+
+  f32x16 oacc[HS / 32], olow[HS / 32];
 #pragma unroll
-  for (int d = 0; d < HS / 32; ++d) oacc[d] = zero16();
+  for (int d = 0; d < HS / 32; ++d) { oacc[d] = zero16(); olow[d] = zero16(); }
   float mb = -INFINITY, l_run = 0.0f;
 
   // Page of a stage's key lane % 32, in wave 0: lanes 0 .. 31 for K, 32 .. 63 for V.
@@ -416,23 +588,52 @@ __global__ __launch_bounds__(256, 2) void paged_prefill_f32_kernel(PrefillArgs<f
     const uint64_t all = __ballot(ok);
     if (tid == 0) holds[stage & 3] = (uint32_t)all;
   };
-  float4 kst[LOADS], vst[LOADS];
-  auto gload = [&](int stage) {
+  auto mask = [&](float (&s)[16], int j0, uint32_t ok) {
+    if (j0 + BN <= v.lo && ~ok == 0) return;
 #pragma unroll
-    for (int u = 0; u < LOADS; ++u) {
-      const int c = tid + 256 * u;
-      kst[u] = ld4(reinterpret_cast<const float*>(row_at[stage & 1][0][c / CH]) + 4 * (c % CH));
-      vst[u] = ld4(reinterpret_cast<const float*>(row_at[stage & 1][1][c / CH]) + 4 * (c % CH));
+    for (int r = 0; r < 16; ++r) {
+      const int j = mfma_row(r, half);
+      if (j0 + j >= v.keys || !(ok >> j & 1)) s[r] = -INFINITY;
+    }
+  };
+
+  // K unit (d8, key), d 8 d8 .. of a key, lies at d8 * 32 + (key ^ (d8 & 7)); V unit (d, sh), the
+  // eight keys that half sh & 1 of the product's step sh >> 1 takes, at (d / 32, sh, d % 32).
+  float kst[NU][8], vst[NU][8];
+  auto gload = [&](int stage) {
+    const uint64_t(*at)[BN] = row_at[stage & 1];
+#pragma unroll
+    for (int u = 0; u < NU; ++u) {
+      const int f = tid + 256 * u;
+      if (UNITS % 256 != 0 && f >= UNITS) continue;  // wave-uniform
+      const float* kp = reinterpret_cast<const float*>(at[0][f / (HS / 8)]) + 8 * (f % (HS / 8));
+      const float4 x = ld4(kp), y = ld4(kp + 4);
+      kst[u][0] = x.x; kst[u][1] = x.y; kst[u][2] = x.z; kst[u][3] = x.w;
+      kst[u][4] = y.x; kst[u][5] = y.y; kst[u][6] = y.z; kst[u][7] = y.w;
+      const int d = f % HS, sh = f / HS, key = 16 * (sh >> 1) + 4 * (sh & 1);
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        vst[u][j] = reinterpret_cast<const float*>(at[1][key + 8 * (j >> 2) + (j & 3)])[d];
     }
   };
   auto lstore = [&](int stage) {
-    float* ks = smem[stage & 1];
-    float* vs = ks + BN * KP;
+    char* ks = smem + (stage & 1) * STAGE;
+    char* vs = ks + 3 * PART;
 #pragma unroll
-    for (int u = 0; u < LOADS; ++u) {
-      const int c = tid + 256 * u;
-      st4(ks + (c / CH) * KP + 4 * (c % CH), kst[u]);
-      st4(vs + (c / CH) * VP + 4 * (c % CH), vst[u]);
+    for (int u = 0; u < NU; ++u) {
+      const int f = tid + 256 * u;
+      if (UNITS % 256 != 0 && f >= UNITS) continue;
+      const int key = f / (HS / 8), d8 = f % (HS / 8);
+      const int d = f % HS, sh = f / HS;
+      bf16x8 p[3];
+      split_bf16(kst[u], p);
+#pragma unroll
+      for (int q = 0; q < 3; ++q)
+        *reinterpret_cast<bf16x8*>(ks + q * PART + (d8 * 32 + (key ^ (d8 & 7))) * 16) = p[q];
+      split_bf16<true>(vst[u], p);
+#pragma unroll
+      for (int q = 0; q < 3; ++q)
+        *reinterpret_cast<bf16x8*>(vs + q * PART + ((d >> 5) * 128 + sh * 32 + (d & 31)) * 16) = p[q];
     }
   };
   if (s_begin < s_end) {  // workgroup-uniform
@@ -446,111 +647,218 @@ __global__ __launch_bounds__(256, 2) void paged_prefill_f32_kernel(PrefillArgs<f
   for (int st = s_begin; st < s_end; ++st) {
     const int page = look_up(st + 2);
     if (st + 1 < s_end) gload(st + 1);
-    const float* ks = smem[st & 1];
-    const float* vs = ks + BN * KP;
+    const char* ks = smem + (st & 1) * STAGE;
+    const char* vs = ks + 3 * PART;
     const int j0 = st * BN;
     if (j0 < v.hi) {  // else no row of this wave sees the stage
-      const uint32_t ok = holds[st & 3];
-      f32x16 acc = zero16();
+      f32x16 acc = zero16(), acc2 = zero16();  // even and odd steps
 #pragma unroll
-      for (int c = 0; c < HS / 8; ++c) {
-        const float4 k4 = ld4(ks + col * KP + 4 * half + 8 * c);
-        acc = mfma32(k4.x, qf[c].x, acc);
-        acc = mfma32(k4.y, qf[c].y, acc);
-        acc = mfma32(k4.z, qf[c].z, acc);
-        acc = mfma32(k4.w, qf[c].w, acc);
+      for (int c = 0; c < HS / 16; c += 2) {
+        bf16x8 ka[2][3];
+#pragma unroll
+        for (int o = 0; o < 2; ++o) {
+          const int d8 = 2 * (c + o) + half;
+          const char* at = ks + (d8 * 32 + (col ^ (d8 & 7))) * 16;
+#pragma unroll
+          for (int q = 2; q >= 0; --q) ka[o][q] = *reinterpret_cast<const bf16x8*>(at + q * PART);
+        }
+#pragma unroll
+        for (int p = 0; p < 6; ++p) {
+          acc = mfma_bf16(ka[0][kSplitA[p]], qp[c][kSplitB[p]], acc);
+          acc2 = mfma_bf16(ka[1][kSplitA[p]], qp[c + 1][kSplitB[p]], acc2);
+        }
       }
       float s[16];
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s[r] = acc[r];
-      exponents(
-          s, a.scale_log2, mb,
-          [&] {
-            if (j0 + BN <= v.lo && ~ok == 0) return;
+      for (int r = 0; r < 16; ++r) s[r] = acc[r] + acc2[r];
+      exponents(s, a.scale_log2 * kSplitUnscale, mb, [&] { mask(s, j0, holds[st & 3]); },
+                [&](float alpha) {
+                  l_run *= alpha;
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-              const int j = mfma_row(r, half);
-              if (j0 + j >= v.keys || !(ok >> j & 1)) s[r] = -INFINITY;
-            }
-          },
-          [&](float alpha) {
-            l_run *= alpha;
-#pragma unroll
-            for (int d = 0; d < HS / 32; ++d) oacc[d] *= alpha;
-          });
+                  for (int d = 0; d < HS / 32; ++d) { oacc[d] *= alpha; olow[d] *= alpha; }
+                });
       l_run += exp2_sum<16>(s);
 #pragma unroll
-      for (int r = 0; r < 16; ++r)
+      for (int i = 0; i < 2; ++i) {  // 16 keys
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = s[8 * i + e];
+        bf16x8 pp[3], va[HS / 32][3];
 #pragma unroll
         for (int d = 0; d < HS / 32; ++d)
-          oacc[d] = mfma32(vs[mfma_row(r, half) * VP + col + 32 * d], s[r], oacc[d]);
+#pragma unroll
+          for (int q = 2; q >= 0; --q)
+            va[d][q] = *reinterpret_cast<const bf16x8*>(
+                vs + q * PART + (d * 128 + (2 * i + half) * 32 + col) * 16);
+        split_bf16<true>(x, pp);
+#pragma unroll
+        for (int p = 0; p < 6; ++p)
+#pragma unroll
+          for (int d = 0; d < HS / 32; ++d) {
+            f32x16& c = p == 5 ? oacc[d] : olow[d];
+            c = mfma_bf16(va[d][kSplitA[p]], pp[kSplitB[p]], c);
+          }
+      }
     }
     if (st + 1 < s_end) lstore(st + 1);
     put(st + 2, page);
     __syncthreads();
   }
-  store_rows<float, HS>(a, w, v, oacc, mb, l_run, half);
-}
 
-// Joins the splits' parts of each row in order; padding rows.  A thread takes four elements.
-template <class E, int HS>
-__global__ __launch_bounds__(256) void paged_prefill_join_kernel(PrefillArgs<E> a, PagedPlan plan) {
-  const int64_t rows = (int64_t)a.N * a.nh;
-  const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int64_t row = id / (HS / 4);
-  const int d = 4 * (int)(id % (HS / 4));
-  if (row >= rows) return;
-  const int t = (int)(row / a.nh);
-  const bool padding = t < plan.cu_q[0] || t >= plan.cu_q[plan.B];
-  const float2* ml = reinterpret_cast<const float2*>(a.ws + a.splits * rows * HS);
-  float m = -INFINITY, l = 0.0f;
-  float4 o = zero4();
-  if (!padding) {
-    for (int s = 0; s < a.splits; ++s) m = fmaxf(m, ml[s * rows + row].x);
-    const float off = m == -INFINITY ? 0.0f : m;
-    for (int s = 0; s < a.splits; ++s) {
-      const float2 p = ml[s * rows + row];
-      const float f = fast_exp2(p.x - off);
-      const float4 v = ld4(a.ws + (s * rows + row) * HS + d);
-      l = fmaf(f, p.y, l);
-      o.x = fmaf(f, v.x, o.x); o.y = fmaf(f, v.y, o.y);
-      o.z = fmaf(f, v.z, o.z); o.w = fmaf(f, v.w, o.w);
+  odd |= !(l_run < INFINITY);
+#pragma unroll
+  for (int d = 0; d < HS / 32; ++d) {
+    oacc[d] += olow[d];
+    odd |= not_finite(oacc[d]);
+    oacc[d] *= kSplitUnscale * kSplitUnscale;
+  }
+  if (__syncthreads_or(odd)) {
+    float* const ks = reinterpret_cast<float*>(smem);
+    float* const vs = ks + BN * KP;
+    mb = -INFINITY;
+    l_run = 0.0f;
+#pragma unroll
+    for (int d = 0; d < HS / 32; ++d) oacc[d] = zero16();
+    for (int st = s_begin; st < s_end; ++st) {
+      put(st, look_up(st));
+      __syncthreads();
+      for (int f = tid; f < BN * HS / 4; f += 256) {
+        const int r = f / (HS / 4), c = f % (HS / 4) * 4;
+        st4(ks + r * KP + c, ld4(reinterpret_cast<const float*>(row_at[st & 1][0][r]) + c));
+        st4(vs + r * VP + c, ld4(reinterpret_cast<const float*>(row_at[st & 1][1][r]) + c));
+      }
+      __syncthreads();
+      const int j0 = st * BN;
+      if (j0 < v.hi) {
+        f32x16 acc = zero16();
+#pragma unroll 2
+        for (int c = 0; c < HS / 8; ++c) {
+          const float4 x = ld4(qrow + 8 * c + 4 * half), y = ld4(ks + col * KP + 8 * c + 4 * half);
+          acc = mfma32(y.x, x.x, acc);
+          acc = mfma32(y.y, x.y, acc);
+          acc = mfma32(y.z, x.z, acc);
+          acc = mfma32(y.w, x.w, acc);
+        }
+        float s[16];
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = acc[r];
+        exponents(s, a.scale_log2, mb, [&] { mask(s, j0, holds[st & 3]); }, [&](float alpha) {
+          l_run *= alpha;
+#pragma unroll
+          for (int d = 0; d < HS / 32; ++d) oacc[d] *= alpha;
+        });
+        l_run += exp2_sum<16>(s);
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+#pragma unroll
+          for (int d = 0; d < HS / 32; ++d)
+            oacc[d] = mfma32(vs[mfma_row(r, half) * VP + col + 32 * d], s[r], oacc[d]);
+      }
+      __syncthreads();
     }
   }
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-  E* op = a.o + row * HS + d;
-  op[0] = (E)(o.x * inv); op[1] = (E)(o.y * inv);
-  op[2] = (E)(o.z * inv); op[3] = (E)(o.w * inv);
-  if (d == 0) a.l[row] = l == 0.0f ? -INFINITY : m * kLn2 + logf(l);
+  store_rows<float, HS>(a, w, slot, oacc, mb, l_run, s_begin < s_end);
+  });
 }
 
-// Tiles of 128 rows a key/value head may have (each sequence may end inside one), one more than
-// that so that some workgroup is left for padding rows; and how many workgroups share a tile's keys:
-// as many as fill the GPU's 512 places, eight stages of 64 keys or more each.
+// Joins the parts of the tiles that several workgroups share, in order, and fills padding rows.  A
+// workgroup has 1024 / HS rows of a tile, a thread four elements of a row.
+template <class E, int HS>
+__global__ __launch_bounds__(256) void paged_prefill_join_kernel(PrefillArgs<E> a, PagedPlan plan) {
+  constexpr int BLOCKS = BM * HS / 1024;  // a tile
+  const int x = blockIdx.x / (BLOCKS * a.nkv), rest = blockIdx.x - x * BLOCKS * a.nkv;
+  RowTile w;
+  w.kvh = rest / BLOCKS;
+  int64_t before;
+  if (!find_rows(a, plan, x, w, before)) {
+    const int base = (int)min(before, (int64_t)a.tiles - 1);
+    fill_padding<E, HS>(a, plan, w.kvh, BLOCKS * (x - base) + rest % BLOCKS, BLOCKS * (a.tiles - base));
+    return;
+  }
+  int64_t front;
+  const Deal deal = make_deal(a, plan, w.b, front);
+  const int64_t begin = w.kvh * deal.head + front + (w.cost - BM * (int64_t)(w.tile + 1)) * w.tile +
+                        BM / 2 * (int64_t)w.tile * (w.tile + 1);
+  const int64_t edge = deal.edge(w.cost);
+  const int w0 = deal.owner(begin + edge), w1 = deal.owner(begin + w.cost - edge - 1);
+  if (w0 == w1) return;  // written whole
+  const int r = 1024 / HS * (rest % BLOCKS) + threadIdx.x / (HS / 4), d = 4 * (threadIdx.x % (HS / 4));
+  if (w.tile * BM + r >= w.R) return;
+  const float2* ml = reinterpret_cast<const float2*>(a.ws + (int64_t)2 * a.W * BM * HS);
+  auto at = [&](int i) { return (int64_t)(2 * i + (i == w0)) * BM + r; };
+  // four parts' loads in flight at a time
+  float m = -INFINITY;
+  for (int i = w0; i <= w1; i += 4) {
+    float x4[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x4[j] = ml[at(min(i + j, w1))].x;
+    m = fmaxf(m, max3_tree(x4));
+  }
+  const float off = m == -INFINITY ? 0.0f : m;
+  float l = 0.0f;
+  float4 o = zero4();
+  for (int i = w0; i <= w1; i += 4) {
+    float2 p[4];
+    float4 v[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      p[j] = ml[at(min(i + j, w1))];
+      v[j] = ld4(a.ws + at(min(i + j, w1)) * HS + d);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      // a share without stages has written no O
+      if (i + j > w1 || (p[j].x == -INFINITY && p[j].y == 0.0f)) continue;
+      const float f = fast_exp2(p[j].x - off);
+      l = fmaf(f, p[j].y, l);
+      o.x = fmaf(f, v[j].x, o.x); o.y = fmaf(f, v[j].y, o.y);
+      o.z = fmaf(f, v[j].z, o.z); o.w = fmaf(f, v[j].w, o.w);
+    }
+  }
+  int token, head;
+  row_of(a, w, w.tile * BM + r, token, head);
+  const int64_t to = (int64_t)token * a.nh + head;
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  E* op = a.o + to * HS + d;
+  op[0] = (E)(o.x * inv); op[1] = (E)(o.y * inv);
+  op[2] = (E)(o.z * inv); op[3] = (E)(o.w * inv);
+  if (d == 0) a.l[to] = l == 0.0f ? -INFINITY : m * kLn2 + logf(l);
+}
+
+// Tiles of 128 rows that a key/value head may have (each sequence may end inside one; one more, so
+// that some workgroup is left for padding rows), and the workgroups that their cost is dealt to: as
+// many as the GPU holds at once, two stages or more each.  From four tiles a place on, or where no
+// tile has more than eight stages, a workgroup takes a whole tile (W = 0).
 struct PrefillGrid {
   int64_t tiles;
-  int splits;
+  int W, stage;
 };
-PrefillGrid prefill_grid(int64_t B, int64_t N, int64_t nh, int64_t nkv, int64_t capacity) {
+PrefillGrid prefill_grid(int64_t B, int64_t N, int64_t nh, int64_t nkv, int64_t hs, int64_t capacity,
+                         int elem) {
   PrefillGrid g;
   g.tiles = N * (nh / nkv) / 128 + std::min(B, N) + 1;
-  const int64_t about = std::max<int64_t>(1, (N * (nh / nkv) + 64 * std::min(B, N)) / 128);
-  const int64_t fill = 512 / (about * nkv);
-  g.splits = (int)std::max<int64_t>(1, std::min<int64_t>({fill, capacity / 512, 16}));
+  g.stage = elem == 4 ? 32 : 64;
+  const int64_t places = 256 * (elem == 4 ? (hs == 128 ? 1 : 2) : (hs == 32 ? 3 : 2));
+  const int64_t about = std::max<int64_t>(1, (N * (nh / nkv) + 64 * std::min(B, N)) / 128) * nkv;
+  const int64_t stages = (capacity + g.stage - 1) / g.stage;
+  g.W = about >= 4 * places || stages <= 8 ? 0 : (int)std::min(places, (g.tiles - 1) * nkv * stages / 2);
   return g;
 }
 
 template <class E, int HS>
 void launch_prefill(const PrefillArgs<E>& a, const PagedPlan& plan, hipStream_t st) {
-  const dim3 grid((unsigned)((int64_t)a.tiles * a.nkv * a.splits));
-  if constexpr (sizeof(E) == 4)
-    hipLaunchKernelGGL((paged_prefill_f32_kernel<HS>), grid, dim3(256), 0, st, a, plan);
-  else
-    hipLaunchKernelGGL((paged_prefill_half_kernel<E, HS>), grid, dim3(256), 0, st, a, plan);
-  if (a.splits > 1)
-    hipLaunchKernelGGL((paged_prefill_join_kernel<E, HS>),
-                       dim3((unsigned)(((int64_t)a.N * a.nh * (HS / 4) + 255) / 256)), dim3(256), 0,
-                       st, a, plan);
+  const dim3 grid(a.W > 0 ? xcd_grid(a.W) : (unsigned)((int64_t)a.tiles * a.nkv));
+  auto go = [&]<bool DEAL>() {
+    if constexpr (sizeof(E) == 4)
+      hipLaunchKernelGGL((paged_prefill_f32_kernel<HS, DEAL>), grid, dim3(256), 0, st, a, plan);
+    else
+      hipLaunchKernelGGL((paged_prefill_half_kernel<E, HS, DEAL>), grid, dim3(256), 0, st, a, plan);
+  };
+  if (a.W > 0) go.template operator()<true>();
+  else go.template operator()<false>();
+  if (a.W > 0)
+    hipLaunchKernelGGL((paged_prefill_join_kernel<E, HS>), dim3((unsigned)((int64_t)a.tiles * a.nkv * (BM * HS / 1024))),
+                       dim3(256), 0, st, a, plan);
 }
 
 template <class E, class P>
@@ -562,10 +870,12 @@ int prefill(const P* q, const int64_t* qs, int64_t N, float scale, P* o, float* 
   if (int rc = check_paged_rows(q, qs, N, pa, scale, o, l, sizeof(E), "paged_attention_prefill"))
     return rc;
   if (N * pa.nh == 0) return CTA_OK;
-  const PrefillGrid g = prefill_grid(pa.B, N, pa.nh, pa.nkv, plan.capacity);
-  if (g.tiles * pa.nkv * g.splits >= (int64_t)1 << 31)
+  const PrefillGrid g = prefill_grid(pa.B, N, pa.nh, pa.nkv, pa.hs, plan.capacity, sizeof(E));
+  const double group = (double)(pa.nh / pa.nkv);
+  if (g.tiles * pa.nkv >= (int64_t)1 << 27 ||  // grids, and the work's units in 53 bits
+      (double)g.tiles * pa.nkv * (group * plan.capacity + 128.0 * g.tiles) >= 0x1p53)
     return fail(CTA_ERR_INVALID_ARGUMENT, "size too large");
-  if (g.splits > 1 && (!ws || !aligned16(ws) ||
+  if (g.W > 0 && (!ws || !aligned16(ws) ||
                        ws_bytes < cta_paged_attention_prefill_workspace(
                                       pa.B, N, pa.nh, pa.nkv, pa.hs, pa.pages_per_seq, pa.page_size)))
     return fail(CTA_ERR_INVALID_ARGUMENT, "paged_attention_prefill needs its workspace");
@@ -578,7 +888,7 @@ int prefill(const P* q, const int64_t* qs, int64_t N, float scale, P* o, float* 
   a.N = (int)N; a.nh = (int)pa.nh; a.nkv = (int)pa.nkv;
   a.group = FastDiv((uint32_t)(pa.nh / pa.nkv));
   a.scale_log2 = scale * kLog2e;
-  a.tiles = (int)g.tiles; a.splits = g.splits;
+  a.tiles = (int)g.tiles; a.W = g.W; a.least = 2 * g.stage * (int)a.group.d;
   a.o = reinterpret_cast<E*>(o); a.l = l; a.ws = static_cast<float*>(ws);
   const hipStream_t st = as_stream(stream);
   if (pa.hs == 32) launch_prefill<E, 32>(a, plan, st);
@@ -598,8 +908,11 @@ extern "C" int64_t cta_paged_attention_prefill_workspace(int64_t B, int64_t N, i
   if (B <= 0 || N <= 0 || nh <= 0 || nkv <= 0 || pages_per_seq <= 0 || page_size <= 0 ||
       (hs != 32 && hs != 64 && hs != 128) || pages_per_seq > ((int64_t)1 << 30) / page_size)
     return 0;
-  const PrefillGrid g = prefill_grid(B, N, nh, nkv, pages_per_seq * page_size);
-  return g.splits > 1 ? (int64_t)g.splits * N * nh * (hs + 2) * 4 : 0;
+  int64_t bytes = 0;  // the most that a type needs
+  for (int elem : {2, 4})
+    bytes = std::max(bytes, (int64_t)prefill_grid(B, N, nh, nkv, hs, pages_per_seq * page_size, elem).W * 2 *
+                                128 * (hs + 2) * 4);
+  return bytes;
 }
 
 #define CTA_PAGED_PREFILL(SUFFIX, TYPE, PTR)                                                      \

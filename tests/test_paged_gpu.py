@@ -308,6 +308,49 @@ def test_prefill_scores_of_any_size(cuda, dtype):
     check_prefill(d, cuda, scale=-0.01)
 
 
+@pytest.mark.parametrize("hs", [32, 64, 128])
+@pytest.mark.parametrize("qk,v", [(2.0 ** 60, 1.0), (1.0, 2.0 ** 110), (2.0 ** -70, 2.0 ** -120), (2.0 ** 90, 2.0 ** -60)])
+def test_prefill_fp32_of_any_magnitude(cuda, hs, qk, v):
+    """Keys and values far from one, beyond the range in which FP32 splits into 16-bit parts; queries
+    the other way, so that scores stay ordinary."""
+    d = make(torch.float32, 4, 2, hs, 16, [70, 33], [40, 33], seed=27, garbage=0.0)
+    d["q"], d["k_cache"], d["v_cache"] = d["q"] / qk, d["k_cache"] * qk, d["v_cache"] * v
+    check_prefill(d, cuda)
+    d["q"], d["k_cache"] = d["q"] * qk * qk, d["k_cache"] / qk / qk
+    check_prefill(d, cuda)
+
+
+@pytest.mark.parametrize("dtype", ALL)
+def test_prefill_infinite_and_huge_scores(cuda, dtype):
+    """A key of -inf scores has no weight, rows of only such keys are empty; equal scores of any
+    size give the mean of V; a NaN key spoils its sequence alone."""
+    dt = DTYPES[dtype]
+    d = make(dt, 2, 1, 32, 16, [40, 20], [9, 20], seed=28)
+    d["q"] = d["q"].abs() + 0.1
+    d["k_cache"][d["table"][0, 1], 0, 3] = -torch.inf
+    for i in range(2):
+        d["k_cache"][d["table"][1, i]] = -torch.inf
+    g = to(d, cuda)
+    args = lambda x: (x["q"], x["k_cache"], x["v_cache"], x["table"], x["lens"], x["cu"])  # noqa: E731
+    O, L = ops.paged_attention_prefill(*args(g))
+    assert torch.isfinite(O).all() and torch.isfinite(L[:9]).all()
+    assert (O[9:] == 0).all() and torch.isneginf(L[9:]).all()
+    big = torch.finfo(dt).max / 2 if dtype == "float16" else 1e30
+    g["q"].fill_(big)
+    g["k_cache"].fill_(-1.0)
+    O, L = ops.paged_attention_prefill(*args(g))
+    rows = torch.cat([d["v_cache"][d["table"][0, i], 0] for i in range(3)]).double()
+    for t in range(9):
+        n = 40 - 8 + t
+        tol = torch.finfo(dt).eps * rows[:n].abs().mean(0).max() + n * 2.0 ** -23
+        assert ((O[t].cpu().double() - rows[:n].mean(0)).abs() <= tol).all()
+    assert torch.isfinite(L).all()
+    g = to(d, cuda)
+    g["k_cache"][g["table"][0, 0], 0, 0, 0] = torch.nan
+    O, L = ops.paged_attention_prefill(*args(g))
+    assert torch.isnan(O[:9]).all() and not torch.isnan(O[9:]).any()
+
+
 @pytest.mark.parametrize("dtype", ALL)
 def test_prefill_strided(cuda, dtype):
     d = to(make(DTYPES[dtype], 6, 2, 64, 16, [100, 7, 33], [40, 7, 30], seed=26, garbage=1.0), cuda)

@@ -74,16 +74,16 @@ __device__ __forceinline__ int64_t uniform(int64_t v) {
   return (int64_t)((uint64_t)(uint32_t)uniform((int)(v >> 32)) << 32 | (uint32_t)uniform((int)v));
 }
 
-// Work counted in tiles, tiles(b) for sequence b: the host does not know the lengths, so a kernel
-// that shares it out counts them itself, 64 sequences a step.
+// Work counted in units, units(b) for sequence b, in integers T: the host does not know the lengths,
+// so a kernel that shares it out counts them itself, 64 sequences a step, a whole wave at a time.
 //
-// Tiles of all B sequences; before: those of the sequences in front of b.  For a whole wave.
-template <class F>
-__device__ __forceinline__ int64_t count_tiles(int B, int b, int64_t& before, F&& tiles) {
+// Units of all B sequences; before: those of the sequences in front of b.
+template <class T, class F>
+__device__ __forceinline__ T count_units(int B, int b, T& before, F&& units) {
   const int lane = threadIdx.x & 63;
-  int64_t total = 0, front = 0;
+  T total = 0, front = 0;
   for (int i = lane; i < B; i += 64) {
-    const int64_t n = tiles(i);
+    const T n = units(i);
     total += n;
     if (i < b) front += n;
   }
@@ -95,21 +95,27 @@ __device__ __forceinline__ int64_t count_tiles(int B, int b, int64_t& before, F&
   before = uniform(front);
   return uniform(total);
 }
-// Sequence that holds tile x of all tiles in a row, and the tiles before it; B, and all tiles, if
-// there are no more than x.  For a whole wave.
-template <class F>
-__device__ __forceinline__ int find_tile(int B, int64_t x, int64_t& before, F&& tiles) {
+// Sums of the lanes' values up to and with each lane.
+template <class T>
+__device__ __forceinline__ T wave_scan(T v) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const T o = __shfl_up(v, off);
+    if (lane >= off) v += o;
+  }
+  return v;
+}
+// Sequence that holds unit x of all units in a row, and the units before it; B, and all units, if
+// there are no more than x.
+template <class T, class F>
+__device__ __forceinline__ int find_unit(int B, T x, T& before, F&& units) {
   const int lane = threadIdx.x & 63;
   before = 0;
   for (int i0 = 0; i0 < B; i0 += 64) {
     const int i = i0 + lane;
-    const int64_t n = i < B ? tiles(i) : 0;
-    int64_t end = n;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-      const int64_t o = __shfl_up(end, off);
-      if (lane >= off) end += o;
-    }
+    const T n = i < B ? (T)units(i) : (T)0;
+    const T end = wave_scan(n);
     const uint64_t past = __ballot(before + end > x);
     if (past) {
       const int w = __builtin_ctzll(past);

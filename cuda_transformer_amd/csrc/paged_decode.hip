@@ -75,13 +75,54 @@ __device__ __forceinline__ f32x4 mfma16(float a, float b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
 }
 
-// Tiles of sequence b.
-template <int TILE>
-__device__ __forceinline__ int tiles_of(const PagedPlan& plan, int b) {
-  return (plan.keys_to((int64_t)plan.lens[b] - 1) + TILE - 1) / TILE;
-}
-// First unit of workgroup w of W <= units: each has at least one.
-__device__ __forceinline__ int64_t deal_start(int64_t units, int w, int W) { return units * w / W; }
+// The deal of all sequences' tiles, `jobs` times over, to W workgroups: units / W each, the first
+// `more` workgroups one more.
+struct Deal {
+  int units, W, each, more;
+  __device__ __forceinline__ Deal(int units_, int grid) : units(units_), W(max(1, min(units_, grid))) {
+    each = (int)((unsigned)units / (unsigned)W);
+    more = units - each * W;
+  }
+  __device__ __forceinline__ int start(int w) const { return w * each + min(w, more); }
+  __device__ __forceinline__ int owner(int u) const {  // the workgroup that has unit u
+    const int cut = more * (each + 1);
+    return u < cut ? (int)((unsigned)u / (unsigned)(each + 1)) : more + (int)((unsigned)(u - cut) / (unsigned)each);
+  }
+};
+// Keys of the sequences.  Up to 64 of them are looked up once, a sequence a lane.
+struct SeqKeys {
+  int lane_keys;
+  bool few;
+  __device__ __forceinline__ explicit SeqKeys(const PagedPlan& plan) : few(plan.B <= 64) {
+    const int lane = threadIdx.x & 63;
+    lane_keys = few && lane < plan.B ? keys(plan, lane) : 0;
+  }
+  static __device__ __forceinline__ int keys(const PagedPlan& plan, int b) {
+    return plan.keys_to((int64_t)plan.lens[b] - 1);
+  }
+  __device__ __forceinline__ int of(const PagedPlan& plan, int b) const {
+    return few ? __builtin_amdgcn_readlane(lane_keys, b) : uniform(keys(plan, b));
+  }
+  // Tiles of all sequences, and of those in front of b.
+  template <int TILE>
+  __device__ __forceinline__ int count(const PagedPlan& plan, int b, int& before) const {
+    if (!few)
+      return count_units(plan.B, b, before, [&](int i) { return (keys(plan, i) + TILE - 1) / TILE; });
+    const int end = wave_scan((lane_keys + TILE - 1) / TILE);
+    before = b == 0 ? 0 : __builtin_amdgcn_readlane(end, b - 1);
+    return __builtin_amdgcn_readlane(end, 63);
+  }
+  // Sequence of tile x, and the tiles before it.
+  template <int TILE>
+  __device__ __forceinline__ int find(const PagedPlan& plan, int x, int& before) const {
+    if (!few)
+      return find_unit(plan.B, x, before, [&](int i) { return (keys(plan, i) + TILE - 1) / TILE; });
+    const int n = (lane_keys + TILE - 1) / TILE, end = wave_scan(n);
+    const int w = __builtin_ctzll(__ballot(end > x));
+    before = __builtin_amdgcn_readlane(end - n, w);
+    return w;
+  }
+};
 
 template <class E, int HS, bool UNIFORM>
 __global__ __launch_bounds__(256, 2) void paged_decode_kernel(DecodeArgs<E> a, PagedPlan plan,
@@ -98,33 +139,31 @@ __global__ __launch_bounds__(256, 2) void paged_decode_kernel(DecodeArgs<E> a, P
   const int col = lane & 15, quarter = lane >> 4;
   const int jobs = a.nkv * a.chunks;  // jobs a sequence
 
-  int64_t u = 0, u_end = 0;
-  int b, job, t, n_tiles;
+  const SeqKeys seqs(plan);
+  int u = 0, u_end, b, job, t, keys, n_tiles;
   if (direct) {
     b = blockIdx.x / jobs;
     job = blockIdx.x - b * jobs;
     t = 0;
-    n_tiles = tiles_of<TILE>(plan, b);
-    u_end = n_tiles;
+    keys = uniform(SeqKeys::keys(plan, b));
+    u_end = n_tiles = (keys + TILE - 1) / TILE;
   } else {
-    int64_t before;
-    auto tiles = [&](int i) { return tiles_of<TILE>(plan, i); };
-    const int64_t units = count_tiles(plan.B, 0, before, tiles) * jobs;
-    const int W = (int)min(units, (int64_t)gridDim.x);
-    if ((int)blockIdx.x >= W) return;
-    u = deal_start(units, blockIdx.x, W);
-    u_end = deal_start(units, blockIdx.x + 1, W);
-    b = find_tile(plan.B, u / jobs, before, tiles);
-    n_tiles = tiles_of<TILE>(plan, b);
-    const int64_t in_seq = u - before * jobs;
-    job = (int)(in_seq / n_tiles);
-    t = (int)(in_seq - (int64_t)job * n_tiles);
+    int before;
+    const Deal deal(seqs.count<TILE>(plan, 0, before) * jobs, gridDim.x);
+    if ((int)blockIdx.x >= deal.W || deal.units == 0) return;
+    u = deal.start(blockIdx.x);
+    u_end = deal.start(blockIdx.x + 1);
+    b = seqs.find<TILE>(plan, (int)((unsigned)u / (unsigned)jobs), before);
+    keys = seqs.of(plan, b);
+    n_tiles = (keys + TILE - 1) / TILE;
+    const int in_seq = u - before * jobs;
+    job = (int)((unsigned)in_seq / (unsigned)n_tiles);
+    t = in_seq - job * n_tiles;
   }
 
   for (;;) {
     // ---- one job, tiles [t, t_end)
-    const int t_end = (int)min((int64_t)n_tiles, t + (u_end - u));
-    const int keys = plan.keys_to((int64_t)plan.lens[b] - 1);
+    const int t_end = min(n_tiles, t + (u_end - u));
     const int kvh = job / a.chunks, chunk = job - kvh * a.chunks;
     const int head0 = kvh * a.group + 16 * chunk, heads = min(16, a.group - 16 * chunk);
     const int32_t* table = plan.table + b * plan.table_stride;
@@ -413,62 +452,92 @@ __global__ __launch_bounds__(256, 2) void paged_decode_kernel(DecodeArgs<E> a, P
     t = 0;
     if (++job == jobs) {
       job = 0;
-      do n_tiles = tiles_of<TILE>(plan, ++b); while (n_tiles == 0);
+      do keys = seqs.of(plan, ++b); while (keys == 0);
+      n_tiles = (keys + TILE - 1) / TILE;
     }
   }
 }
 
-// Joins the parts of the jobs that several workgroups of W share; rows without a key.  One workgroup
-// for each sequence and query head; its threads take an element of the row and every PG-th part.
-template <class E, int HS>
+// Joins the parts of the jobs that several workgroups share, in order of groups of parts; rows without
+// a key.  WAVES waves have a row of O (a sequence and query head), HS / 4 lanes a part of it.
+template <class E, int HS, int WAVES>
 __global__ __launch_bounds__(256) void paged_decode_join_kernel(DecodeArgs<E> a, PagedPlan plan,
                                                                 int grid) {
   using D = DecodeTile<E, HS>;
-  constexpr int PG = 256 / HS;
-  __shared__ float xo[PG][HS], xl[PG];
-  const int b = blockIdx.x / a.nh, h = blockIdx.x - b * a.nh;
+  constexpr int LP = HS / 4, PG = 64 / LP;  // lanes a part; parts a wave takes at a time
+  __shared__ __attribute__((aligned(16))) float xo[WAVES][HS];
+  __shared__ float xm[WAVES], xl[WAVES];
+  const int lane = threadIdx.x & 63, wave = wave_index();
+  const int id = blockIdx.x * (4 / WAVES) + wave / WAVES;
+  const bool live = id < plan.B * a.nh;  // idle waves of the last workgroup stay for the barrier
+  const int b = live ? id / a.nh : 0, h = live ? id - b * a.nh : 0;
   const int kvh = h / a.group, in_group = h - kvh * a.group;
   const int job = kvh * a.chunks + in_group / 16, row = in_group % 16;
   const int jobs = a.nkv * a.chunks;
-  int64_t before;
-  const int64_t units =
-      count_tiles(plan.B, b, before, [&](int i) { return tiles_of<D::TILE>(plan, i); }) * jobs;
-  const int n = tiles_of<D::TILE>(plan, b);
-  const int64_t at = (int64_t)b * a.nh + h;
-  const int d = threadIdx.x % HS, pg = threadIdx.x / HS;
-  if (n == 0) {
-    if (pg == 0) a.o[at * HS + d] = (E)0.0f;
-    if (threadIdx.x == 0) a.l[at] = -INFINITY;
-    return;
+  const SeqKeys seqs(plan);
+  int before;
+  const Deal deal(seqs.count<D::TILE>(plan, b, before) * jobs, grid);
+  const int n = (seqs.of(plan, b) + D::TILE - 1) / D::TILE;
+  int w0 = 0, w1 = -1;
+  if (n > 0) {
+    const int first = before * jobs + job * n;
+    w0 = deal.owner(first);
+    w1 = deal.owner(first + n - 1);
+    if (w0 == w1) return;  // written whole (all waves of the row agree)
   }
-  const int W = (int)min(units, (int64_t)grid);
-  // workgroups of the job's first and last unit: the last w with deal_start(w) <= unit
-  const int64_t first = before * jobs + (int64_t)job * n, last = first + n - 1;
-  auto owner = [&](int64_t unit) { return (int)(((unit + 1) * W - 1) / units); };
-  const int w0 = owner(first), w1 = owner(last);
-  if (w0 == w1) return;  // written whole
-  auto part = [&](int w) { return a.ws + ((int64_t)w * 2 + (w == w0)) * D::PART; };
-
-  const int lane = threadIdx.x & 63;
-  float m = -INFINITY;
-  for (int w = w0 + lane; w <= w1; w += 64) m = fmaxf(m, part(w)[16 * HS + row]);
-  m = wave_max(m);
-  const float off = m == -INFINITY ? 0.0f : m;
-  float o = 0.0f, l = 0.0f;
-  for (int w = w0 + pg; w <= w1; w += PG) {
-    const float* p = part(w);
-    const float f = fast_exp2(p[16 * HS + row] - off);
-    l = fmaf(f, p[16 * HS + 16 + row], l);
-    o = fmaf(f, p[row * HS + d], o);
-  }
-  xo[pg][d] = o;
-  if (d == 0) xl[pg] = l;
-  __syncthreads();
-  if (pg != 0) return;
+  if (!live) return;
+  const int d = 4 * (lane % LP);
+  constexpr int STEP = PG * WAVES;
+  float m = -INFINITY, l = 0.0f;
+  float4 o = zero4();
+  for (int w = w0 + lane / LP + PG * (wave % WAVES); w <= w1; w += 2 * STEP) {
+    // two parts' loads in flight
+    float pm[2], pl[2];
+    float4 v[2];
 #pragma unroll
-  for (int i = 1; i < PG; ++i) { o += xo[i][d]; l += xl[i]; }
-  a.o[at * HS + d] = (E)(l == 0.0f ? 0.0f : o / l);
-  if (d == 0) a.l[at] = l == 0.0f ? -INFINITY : off * kLn2 + logf(l);
+    for (int j = 0; j < 2; ++j) {
+      const int i = w + j * STEP <= w1 ? w + j * STEP : w;
+      const float* p = a.ws + ((int64_t)i * 2 + (i == w0)) * D::PART;
+      pm[j] = w + j * STEP <= w1 ? p[16 * HS + row] : -INFINITY;
+      pl[j] = p[16 * HS + 16 + row];
+      v[j] = ld4(p + row * HS + d);
+    }
+    const float m_new = fmaxf(m, fmaxf(pm[0], pm[1])), off = m_new == -INFINITY ? 0.0f : m_new;
+    const float f = fast_exp2(m - off), f0 = fast_exp2(pm[0] - off), f1 = fast_exp2(pm[1] - off);
+    l = l * f + (pl[0] * f0 + pl[1] * f1);
+    o.x = o.x * f + (v[0].x * f0 + v[1].x * f1);
+    o.y = o.y * f + (v[0].y * f0 + v[1].y * f1);
+    o.z = o.z * f + (v[0].z * f0 + v[1].z * f1);
+    o.w = o.w * f + (v[0].w * f0 + v[1].w * f1);
+    m = m_new;
+  }
+  auto join = [&](float m2, float l2, float4 o2) {
+    const float m_new = fmaxf(m, m2), off = m_new == -INFINITY ? 0.0f : m_new;
+    const float f = fast_exp2(m - off), f2 = fast_exp2(m2 - off);
+    l = l * f + l2 * f2;
+    o.x = o.x * f + o2.x * f2; o.y = o.y * f + o2.y * f2;
+    o.z = o.z * f + o2.z * f2; o.w = o.w * f + o2.w * f2;
+    m = m_new;
+  };
+#pragma unroll
+  for (int x = LP; x < 64; x <<= 1)
+    join(__shfl_xor(m, x), __shfl_xor(l, x),
+         make_float4(__shfl_xor(o.x, x), __shfl_xor(o.y, x), __shfl_xor(o.z, x), __shfl_xor(o.w, x)));
+  if constexpr (WAVES > 1) {
+    if (lane < LP) st4(&xo[wave][d], o);
+    if (lane == 0) { xm[wave] = m; xl[wave] = l; }
+    __syncthreads();
+    if (wave > 0) return;
+#pragma unroll
+    for (int x = 1; x < WAVES; ++x) join(xm[x], xl[x], ld4(&xo[x][d]));
+  }
+  if (lane >= LP) return;
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  const int64_t at = (int64_t)b * a.nh + h;
+  E* op = a.o + at * HS + d;
+  op[0] = (E)(o.x * inv); op[1] = (E)(o.y * inv);
+  op[2] = (E)(o.z * inv); op[3] = (E)(o.w * inv);
+  if (lane == 0) a.l[at] = l == 0.0f ? -INFINITY : m * kLn2 + logf(l);
 }
 
 // Workgroups that the tiles are dealt to, or 0 where every job is one workgroup's (direct).
@@ -493,8 +562,13 @@ void launch_decode(const DecodeArgs<E>& a, const PagedPlan& plan, const DecodeGr
     hipLaunchKernelGGL((paged_decode_kernel<E, HS, true>), grid, dim3(256), 0, st, a, plan, g.W == 0);
   else
     hipLaunchKernelGGL((paged_decode_kernel<E, HS, false>), grid, dim3(256), 0, st, a, plan, g.W == 0);
-  if (g.W > 0)
-    hipLaunchKernelGGL((paged_decode_join_kernel<E, HS>), dim3((unsigned)(plan.B * a.nh)), dim3(256), 0, st, a, plan, g.W);
+  if (g.W == 0) return;
+  const int64_t rows = (int64_t)plan.B * a.nh;
+  // four waves a row where a job has eight parts or more on average
+  if (g.W >= 8 * g.jobs)
+    hipLaunchKernelGGL((paged_decode_join_kernel<E, HS, 4>), dim3((unsigned)rows), dim3(256), 0, st, a, plan, g.W);
+  else
+    hipLaunchKernelGGL((paged_decode_join_kernel<E, HS, 1>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, a, plan, g.W);
 }
 
 template <class E, class P>
@@ -506,6 +580,8 @@ int decode(const P* q, const int64_t* qs, float scale, P* o, float* l, void* ws,
     return rc;
   if (pa.B * pa.nh == 0) return CTA_OK;
   const DecodeGrid g = decode_grid(pa.B, pa.nh, pa.nkv, pa.hs, plan.capacity, sizeof(E));
+  if ((double)g.jobs * (plan.capacity / tile_keys(pa.hs, sizeof(E)) + 1) >= 0x1p31)  // tiles dealt
+    return fail(CTA_ERR_INVALID_ARGUMENT, "size too large");
   if (g.W > 0 && (!ws || !aligned16(ws) ||
                   ws_bytes < cta_paged_attention_decode_workspace(pa.B, pa.nh, pa.nkv, pa.hs,
                                                                   pa.pages_per_seq, pa.page_size)))

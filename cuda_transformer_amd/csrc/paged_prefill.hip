@@ -86,7 +86,7 @@ __device__ __forceinline__ SeqCost seq_cost(const PrefillArgs<E>& a, const Paged
 template <class E>
 __device__ __forceinline__ bool find_rows(const PrefillArgs<E>& a, const PagedPlan& plan, int x,
                                           RowTile& w, int64_t& before) {
-  w.b = find_tile(plan.B, x, before, [&](int i) { return (int64_t)seq_cost(a, plan, i).tiles(); });
+  w.b = find_unit(plan.B, (int64_t)x, before, [&](int i) { return seq_cost(a, plan, i).tiles(); });
   if (w.b == plan.B) return false;
   const SeqCost c = seq_cost(a, plan, w.b);
   w.first = uniform(c.first);
@@ -113,7 +113,7 @@ template <class E>
 __device__ __forceinline__ Deal make_deal(const PrefillArgs<E>& a, const PagedPlan& plan, int b,
                                           int64_t& before) {
   Deal d;
-  d.head = count_tiles(plan.B, b, before, [&](int i) {
+  d.head = count_units(plan.B, b, before, [&](int i) {
     const SeqCost c = seq_cost(a, plan, i);
     return c.upto(c.tiles());
   });
@@ -124,12 +124,12 @@ __device__ __forceinline__ Deal make_deal(const PrefillArgs<E>& a, const PagedPl
 }
 // The tile that holds unit u, which is made relative to the tile's begin.
 template <class E>
-__device__ __forceinline__ void find_unit(const PrefillArgs<E>& a, const PagedPlan& plan,
-                                          const Deal& d, int64_t& u, RowTile& w) {
+__device__ __forceinline__ void find_share(const PrefillArgs<E>& a, const PagedPlan& plan,
+                                           const Deal& d, int64_t& u, RowTile& w) {
   w.kvh = (int)(u / d.head);
   u -= w.kvh * d.head;
   int64_t before;
-  w.b = find_tile(plan.B, u, before, [&](int i) {
+  w.b = find_unit(plan.B, u, before, [&](int i) {
     const SeqCost c = seq_cost(a, plan, i);
     return c.upto(c.tiles());
   });
@@ -205,7 +205,7 @@ __device__ __forceinline__ void each_tile(const PrefillArgs<E>& a, const PagedPl
     int64_t u = deal.cut(n);
     int64_t left = deal.cut(n + 1) - u;  // units from the tile's begin to this workgroup's end
     if (left == 0) return;
-    find_unit(a, plan, deal, u, w);
+    find_share(a, plan, deal, u, w);
     left += u;
     w.lo = u <= deal.edge(w.cost) ? 0 : u;
     if (u >= w.cost - deal.edge(w.cost)) {  // the share begins at the next tile

@@ -7,9 +7,9 @@
 // against the largest m_i.
 //
 // What bounds it: every key and value is read once, 2 group to 4 group operations a byte.  So the
-// products run on the matrix pipe, whose idle columns cost nothing (16 query heads a pass, whatever
-// the group), and everything else serves the loads.
-//  * A job is one sequence's keys for one key/value head (and 16 of its query heads).  Jobs are cut
+// products run on the matrix pipe, whose idle columns cost nothing (16 query heads a pass, or 32 for
+// groups above 16), and everything else serves the loads.
+//  * A job is one sequence's keys for one key/value head (and 16 or 32 of its query heads).  Jobs are cut
 //    into tiles of 4 x WK keys and all tiles of all jobs are dealt evenly, in order, to a fixed
 //    number of workgroups: lengths that differ by any factor load the GPU evenly.  A workgroup
 //    writes the jobs it has whole, and partial results (at most two: the job it enters in the
@@ -36,15 +36,16 @@ struct DecodeArgs {
   const E *q, *k, *v;
   int64_t qt, qh;
   Strides3 sk, sv;
-  int nh, nkv, group, chunks;  // chunks of 16 query heads a key/value head
+  int nh, nkv, group, chunks;  // chunks of 16 M query heads a key/value head
   float scale_log2;
   E* o;
   float* l;
   float* ws;
 };
 
-// Geometry of a type and head size: 16 KB of K and V a wave and tile.
-template <class E, int HS>
+// Geometry of a type, head size and number M of 16 query heads a pass: 16 KB of K and V a wave and
+// tile.
+template <class E, int HS, int M = 1>
 struct DecodeTile {
   static constexpr int KG = sizeof(E) == 2 ? 256 / HS : 128 / HS;  // groups of 16 keys a wave
   static constexpr int WK = 16 * KG;                               // keys a wave
@@ -52,7 +53,8 @@ struct DecodeTile {
   static constexpr int CK = HS * (int)sizeof(E) / 64;  // 16-byte chunks a lane has of a K row
   static constexpr int DW = HS * (int)sizeof(E) / 64;  // dwords a lane has of a V row
   static constexpr int NE = HS / 16;                   // output elements of a lane and register
-  static constexpr int PART = 16 * (HS + 2);           // floats of a partial result: O, m, l
+  static constexpr int HEADS = 16 * M;
+  static constexpr int PART = HEADS * (HS + 2);        // floats of a partial result: O, m, l
 };
 
 // Largest of the values that lanes l, l ^ 16, l ^ 32, l ^ 48 hold, and their sum.
@@ -124,15 +126,17 @@ struct SeqKeys {
   }
 };
 
-template <class E, int HS, bool UNIFORM>
+// UNIFORM: a group of 16 keys lies in one page (the page size is a multiple of 16).  STREAM: K and V
+// are read past the caches.
+template <class E, int HS, int M, bool UNIFORM, bool STREAM>
 __global__ __launch_bounds__(256, 2) void paged_decode_kernel(DecodeArgs<E> a, PagedPlan plan,
                                                               bool direct) {
-  using D = DecodeTile<E, HS>;
+  using D = DecodeTile<E, HS, M>;
   constexpr int KG = D::KG, WK = D::WK, TILE = D::TILE, CK = D::CK, DW = D::DW, NE = D::NE;
   constexpr bool F32 = sizeof(E) == 4;
   constexpr int OP = HS + 4;  // pitch of a head's row in the exchange
-  __shared__ __attribute__((aligned(16))) float xo[4][16][OP];
-  __shared__ float xm[4][16], xl[4][16];
+  __shared__ __attribute__((aligned(16))) float xo[4][D::HEADS][OP];
+  __shared__ float xm[4][D::HEADS], xl[4][D::HEADS];
   __shared__ int64_t rows_at[UNIFORM ? 1 : 4][2][UNIFORM ? 1 : WK];
 
   const int lane = threadIdx.x & 63, wave = wave_index();
@@ -165,25 +169,29 @@ __global__ __launch_bounds__(256, 2) void paged_decode_kernel(DecodeArgs<E> a, P
     // ---- one job, tiles [t, t_end)
     const int t_end = min(n_tiles, t + (u_end - u));
     const int kvh = job / a.chunks, chunk = job - kvh * a.chunks;
-    const int head0 = kvh * a.group + 16 * chunk, heads = min(16, a.group - 16 * chunk);
+    const int head0 = kvh * a.group + D::HEADS * chunk, heads = min(D::HEADS, a.group - D::HEADS * chunk);
     const int32_t* table = plan.table + b * plan.table_stride;
     const E* kb = a.k + kvh * a.sk.h;
     const E* vb = a.v + kvh * a.sv.h;
 
     // Q in the order of the B operand: column = head, the chunk of d of the K operand
-    u32x4 qf[CK];
+    u32x4 qf[M][CK];
+    f32x4 acc[M][NE];
+    float m[M], l[M];
 #pragma unroll
-    for (int s = 0; s < CK; ++s) {
-      qf[s] = u32x4{0, 0, 0, 0};
-      if (col < heads)
-        qf[s] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const char*>(
-                    a.q + b * a.qt + (head0 + col) * a.qh) + 64 * s + 16 * quarter);
+    for (int i = 0; i < M; ++i) {
+#pragma unroll
+      for (int s = 0; s < CK; ++s) {
+        qf[i][s] = u32x4{0, 0, 0, 0};
+        if (16 * i + col < heads)
+          qf[i][s] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const char*>(
+                         a.q + b * a.qt + (head0 + 16 * i + col) * a.qh) + 64 * s + 16 * quarter);
+      }
+#pragma unroll
+      for (int e = 0; e < NE; ++e) acc[i][e] = f32x4{0, 0, 0, 0};
+      m[i] = -INFINITY;
+      l[i] = 0.0f;
     }
-
-    f32x4 acc[NE];
-#pragma unroll
-    for (int e = 0; e < NE; ++e) acc[e] = f32x4{0, 0, 0, 0};
-    float m = -INFINITY, l = 0.0f;
 
     // Page of this wave's group of 16 keys (UNIFORM): lane i has group i % KG of the i / KG-th tile
     // from tp on.  Entries behind the last key are not read.
@@ -209,6 +217,10 @@ __global__ __launch_bounds__(256, 2) void paged_decode_kernel(DecodeArgs<E> a, P
     bool full_k = false, full_v = false;
     int page_of[KG];  // of the tile whose K was loaded last (UNIFORM)
 
+    auto load = []<class T>(const char* p) {
+      if constexpr (STREAM) return __builtin_nontemporal_load(reinterpret_cast<const T*>(p));
+      else return *reinterpret_cast<const T*>(p);
+    };
     auto load_k = [&](int tile) {
       const int k0 = tile * TILE + wave * WK;
       if constexpr (UNIFORM) {
@@ -233,7 +245,7 @@ __global__ __launch_bounds__(256, 2) void paged_decode_kernel(DecodeArgs<E> a, P
           const int at = col * (int)a.sk.r * (int)sizeof(E) + 16 * quarter;
 #pragma unroll
           for (int s = 0; s < CK; ++s)
-            kr[g][s] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const char*>(p) + (uint32_t)(at + 64 * s));
+            kr[g][s] = load.template operator()<u32x4>(reinterpret_cast<const char*>(p) + (uint32_t)(at + 64 * s));
           if (page_of[g] >= 0)
             valid_k |= (0xfu >> (4 - min(max(keys - key - 4 * quarter, 0), 4))) << (4 * g);
         }
@@ -262,7 +274,7 @@ __global__ __launch_bounds__(256, 2) void paged_decode_kernel(DecodeArgs<E> a, P
           const int64_t at = max(rows_at[wave][0][16 * g + col], (int64_t)0);
 #pragma unroll
           for (int s = 0; s < CK; ++s)
-            kr[g][s] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const char*>(kb + at) + 64 * s + 16 * quarter);
+            kr[g][s] = load.template operator()<u32x4>(reinterpret_cast<const char*>(kb + at) + 64 * s + 16 * quarter);
 #pragma unroll
           for (int r = 0; r < 4; ++r)
             valid_k |= (uint32_t)(rows_at[wave][0][16 * g + 4 * quarter + r] >= 0) << (4 * g + r);
@@ -295,15 +307,15 @@ __global__ __launch_bounds__(256, 2) void paged_decode_kernel(DecodeArgs<E> a, P
           if constexpr (DW >= 4) {
 #pragma unroll
             for (int c = 0; c < DW / 4; ++c) {
-              const u32x4 w = reinterpret_cast<const u32x4*>(src)[c];
+              const u32x4 w = load.template operator()<u32x4>(src + 16 * c);
 #pragma unroll
               for (int i = 0; i < 4; ++i) x[4 * c + i] = w[i];
             }
           } else if constexpr (DW == 2) {
-            const uint2 w = *reinterpret_cast<const uint2*>(src);
-            x[0] = w.x; x[1] = w.y;
+            const u32x2 w = load.template operator()<u32x2>(src);
+            x[0] = w[0]; x[1] = w[1];
           } else {
-            x[0] = *reinterpret_cast<const uint32_t*>(src);
+            x[0] = load.template operator()<uint32_t>(src);
           }
         }
       }
@@ -318,48 +330,56 @@ __global__ __launch_bounds__(256, 2) void paged_decode_kernel(DecodeArgs<E> a, P
       // scores of any size have equal exponents
 #pragma clang fp contract(off)
       // ---- scores of 16 KG keys: lane, register r of group g: key 16 g + 4 quarter + r, head col
-      f32x4 s[KG];
+      f32x4 s[M][KG];
 #pragma unroll
-      for (int g = 0; g < KG; ++g) s[g] = f32x4{0, 0, 0, 0};
+      for (int i = 0; i < M; ++i)
+#pragma unroll
+        for (int g = 0; g < KG; ++g) s[i][g] = f32x4{0, 0, 0, 0};
 #pragma unroll
       for (int c = 0; c < CK; ++c)
 #pragma unroll
-        for (int g = 0; g < KG; ++g) {
-          if constexpr (F32) {
+        for (int g = 0; g < KG; ++g)
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-              s[g] = mfma16(__uint_as_float(kr[g][c][i]), __uint_as_float(qf[c][i]), s[g]);
-          } else {
-            s[g] = mfma16(__builtin_bit_cast(vec8_t<E>, kr[g][c]), __builtin_bit_cast(vec8_t<E>, qf[c]), s[g]);
+          for (int i = 0; i < M; ++i) {
+            if constexpr (F32) {
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                s[i][g] = mfma16(__uint_as_float(kr[g][c][j]), __uint_as_float(qf[i][c][j]), s[i][g]);
+            } else {
+              s[i][g] = mfma16(__builtin_bit_cast(vec8_t<E>, kr[g][c]),
+                               __builtin_bit_cast(vec8_t<E>, qf[i][c]), s[i][g]);
+            }
           }
-        }
       if (tile + 1 < t_end) load_k(tile + 1);
-      float mt = -INFINITY;
 #pragma unroll
-      for (int g = 0; g < KG; ++g)
+      for (int i = 0; i < M; ++i) {
+        float mt = -INFINITY;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          s[g][r] *= a.scale_log2;
-          if (!full_v && !(valid_v >> (4 * g + r) & 1)) s[g][r] = -INFINITY;
-          mt = fmaxf(mt, s[g][r]);
+        for (int g = 0; g < KG; ++g)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            s[i][g][r] *= a.scale_log2;
+            if (!full_v && !(valid_v >> (4 * g + r) & 1)) s[i][g][r] = -INFINITY;
+            mt = fmaxf(mt, s[i][g][r]);
+          }
+        mt = max_quarters(mt);
+        if (__any(mt > m[i])) {
+          const float m_new = fmaxf(m[i], mt);
+          const float alpha = fast_exp2(m[i] - (m_new == -INFINITY ? 0.0f : m_new));
+          l[i] *= alpha;
+#pragma unroll
+          for (int e = 0; e < NE; ++e) acc[i][e] *= alpha;
+          m[i] = m_new;
         }
-      mt = max_quarters(mt);
-      if (__any(mt > m)) {
-        const float m_new = fmaxf(m, mt);
-        const float alpha = fast_exp2(m - (m_new == -INFINITY ? 0.0f : m_new));
-        l *= alpha;
+        const float off = m[i] == -INFINITY ? 0.0f : m[i];
 #pragma unroll
-        for (int e = 0; e < NE; ++e) acc[e] *= alpha;
-        m = m_new;
+        for (int g = 0; g < KG; ++g)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            s[i][g][r] = fast_exp2(s[i][g][r] - off);
+            l[i] += s[i][g][r];
+          }
       }
-      const float off = m == -INFINITY ? 0.0f : m;
-#pragma unroll
-      for (int g = 0; g < KG; ++g)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          s[g][r] = fast_exp2(s[g][r] - off);
-          l += s[g][r];
-        }
       // rows without a key count as zeros: what lies there may be anything
       if (!full_v) {
 #pragma unroll
@@ -377,17 +397,21 @@ __global__ __launch_bounds__(256, 2) void paged_decode_kernel(DecodeArgs<E> a, P
           for (int r = 0; r < 4; ++r)
 #pragma unroll
             for (int e = 0; e < NE; ++e)
-              acc[e] = mfma16(__uint_as_float(vr[4 * g + r][e]), s[g][r], acc[e]);
+#pragma unroll
+              for (int i = 0; i < M; ++i)
+                acc[i][e] = mfma16(__uint_as_float(vr[4 * g + r][e]), s[i][g][r], acc[i][e]);
       } else {
 #pragma unroll
         for (int g = 0; g < KG; g += 2) {  // 32 keys: the lane's 8 are its k-slots
-          vec8_t<E> hi, lo;
+          vec8_t<E> hi[M], lo[M];
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const float p = s[g + (j >> 2)][j & 3];
-            hi[j] = (E)p;
-            lo[j] = (E)(p - (float)hi[j]);
-          }
+          for (int i = 0; i < M; ++i)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              const float p = s[i][g + (j >> 2)][j & 3];
+              hi[i][j] = (E)p;
+              lo[i][j] = (E)(p - (float)hi[i][j]);
+            }
 #pragma unroll
           for (int e = 0; e < NE; ++e) {
             u32x4 w;
@@ -397,8 +421,11 @@ __global__ __launch_bounds__(256, 2) void paged_decode_kernel(DecodeArgs<E> a, P
               w[i] = e % 2 ? pack_hi16(x, y) : pack_lo16(x, y);
             }
             const auto va = __builtin_bit_cast(vec8_t<E>, w);
-            acc[e] = mfma16(va, lo, acc[e]);
-            acc[e] = mfma16(va, hi, acc[e]);
+#pragma unroll
+            for (int i = 0; i < M; ++i) {
+              acc[i][e] = mfma16(va, lo[i], acc[i][e]);
+              acc[i][e] = mfma16(va, hi[i], acc[i][e]);
+            }
           }
         }
       }
@@ -406,12 +433,15 @@ __global__ __launch_bounds__(256, 2) void paged_decode_kernel(DecodeArgs<E> a, P
     }
 
     // ---- the four waves' parts, against the largest offset
-    l = sum_quarters(l);
-    if (quarter == 0) { xm[wave][col] = m; xl[wave][col] = l; }
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
+    for (int i = 0; i < M; ++i) {
+      const float sum = sum_quarters(l[i]);
+      if (quarter == 0) { xm[wave][16 * i + col] = m[i]; xl[wave][16 * i + col] = sum; }
 #pragma unroll
-      for (int e = 0; e < NE; ++e) xo[wave][col][NE * (4 * quarter + r) + e] = acc[e][r];
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int e = 0; e < NE; ++e) xo[wave][16 * i + col][NE * (4 * quarter + r) + e] = acc[i][e][r];
+    }
     __syncthreads();
     const bool whole = t == 0 && t_end == n_tiles;
     // a job that began in an earlier workgroup goes to this one's first slot, else to its second
@@ -442,7 +472,7 @@ __global__ __launch_bounds__(256, 2) void paged_decode_kernel(DecodeArgs<E> a, P
         if (d == 0) a.l[at] = lj == 0.0f ? -INFINITY : off * kLn2 + logf(lj);
       } else {
         st4(part + h * HS + d, o);
-        if (d == 0) { part[16 * HS + h] = mj; part[16 * HS + 16 + h] = lj; }
+        if (d == 0) { part[D::HEADS * HS + h] = mj; part[D::HEADS * (HS + 1) + h] = lj; }
       }
     }
 
@@ -460,10 +490,10 @@ __global__ __launch_bounds__(256, 2) void paged_decode_kernel(DecodeArgs<E> a, P
 
 // Joins the parts of the jobs that several workgroups share, in order of groups of parts; rows without
 // a key.  WAVES waves have a row of O (a sequence and query head), HS / 4 lanes a part of it.
-template <class E, int HS, int WAVES>
+template <class E, int HS, int M, int WAVES>
 __global__ __launch_bounds__(256) void paged_decode_join_kernel(DecodeArgs<E> a, PagedPlan plan,
                                                                 int grid) {
-  using D = DecodeTile<E, HS>;
+  using D = DecodeTile<E, HS, M>;
   constexpr int LP = HS / 4, PG = 64 / LP;  // lanes a part; parts a wave takes at a time
   __shared__ __attribute__((aligned(16))) float xo[WAVES][HS];
   __shared__ float xm[WAVES], xl[WAVES];
@@ -472,7 +502,7 @@ __global__ __launch_bounds__(256) void paged_decode_join_kernel(DecodeArgs<E> a,
   const bool live = id < plan.B * a.nh;  // idle waves of the last workgroup stay for the barrier
   const int b = live ? id / a.nh : 0, h = live ? id - b * a.nh : 0;
   const int kvh = h / a.group, in_group = h - kvh * a.group;
-  const int job = kvh * a.chunks + in_group / 16, row = in_group % 16;
+  const int job = kvh * a.chunks + in_group / D::HEADS, row = in_group % D::HEADS;
   const int jobs = a.nkv * a.chunks;
   const SeqKeys seqs(plan);
   int before;
@@ -498,8 +528,8 @@ __global__ __launch_bounds__(256) void paged_decode_join_kernel(DecodeArgs<E> a,
     for (int j = 0; j < 2; ++j) {
       const int i = w + j * STEP <= w1 ? w + j * STEP : w;
       const float* p = a.ws + ((int64_t)i * 2 + (i == w0)) * D::PART;
-      pm[j] = w + j * STEP <= w1 ? p[16 * HS + row] : -INFINITY;
-      pl[j] = p[16 * HS + 16 + row];
+      pm[j] = w + j * STEP <= w1 ? p[D::HEADS * HS + row] : -INFINITY;
+      pl[j] = p[D::HEADS * (HS + 1) + row];
       v[j] = ld4(p + row * HS + d);
     }
     const float m_new = fmaxf(m, fmaxf(pm[0], pm[1])), off = m_new == -INFINITY ? 0.0f : m_new;
@@ -540,35 +570,49 @@ __global__ __launch_bounds__(256) void paged_decode_join_kernel(DecodeArgs<E> a,
   if (lane == 0) a.l[at] = l == 0.0f ? -INFINITY : m * kLn2 + logf(l);
 }
 
-// Workgroups that the tiles are dealt to, or 0 where every job is one workgroup's (direct).
+// How a call is laid out.  pass: query heads that a pass over K and V serves (16 M).  W: workgroups
+// that the tiles are dealt to, two a CU, or 0 where every job is one workgroup's (direct): up to four
+// tiles a job are walked in the time that the second kernel takes.
 struct DecodeGrid {
-  int64_t jobs;
-  int W;
+  int64_t chunks, jobs;
+  int pass, W;
 };
 int tile_keys(int64_t hs, int elem) { return (int)(4 * 16 * (elem == 2 ? 256 / hs : 128 / hs)); }
 DecodeGrid decode_grid(int64_t B, int64_t nh, int64_t nkv, int64_t hs, int64_t capacity, int elem) {
   DecodeGrid g;
-  g.jobs = B * nkv * ((nh / nkv + 15) / 16);
+  g.pass = nh / nkv > 16 ? 32 : 16;
+  g.chunks = (nh / nkv + g.pass - 1) / g.pass;
+  g.jobs = B * nkv * g.chunks;
   const int64_t tiles = (capacity + tile_keys(hs, elem) - 1) / tile_keys(hs, elem);
-  // Up to four tiles a job are walked in the time that the second kernel takes.
   g.W = tiles <= 4 ? 0 : (int)std::min<int64_t>(g.jobs * tiles, 512);
   return g;
 }
 
-template <class E, int HS>
-void launch_decode(const DecodeArgs<E>& a, const PagedPlan& plan, const DecodeGrid& g, hipStream_t st) {
+// Pools from this size on are read past the caches, unless several chunks of heads read the same
+// keys: four layers of them exceed the 256 MB last-level cache, so nothing is left of a layer's keys
+// when the next token reads them.  64 sequences of 500 to 8000 tokens (743 MB): 140 us through the
+// caches, 124 past them; 16 of 200 to 1000 (37 MB, read again while still cached): 15.1 and 15.9.
+constexpr int64_t kStreamBytes = (int64_t)64 << 20;
+
+template <class E, int HS, int M>
+void launch_decode(const DecodeArgs<E>& a, const PagedPlan& plan, const DecodeGrid& g, bool stream,
+                   hipStream_t st) {
   const dim3 grid((unsigned)(g.W > 0 ? g.W : g.jobs));
-  if (plan.ps.d % 16 == 0)
-    hipLaunchKernelGGL((paged_decode_kernel<E, HS, true>), grid, dim3(256), 0, st, a, plan, g.W == 0);
-  else
-    hipLaunchKernelGGL((paged_decode_kernel<E, HS, false>), grid, dim3(256), 0, st, a, plan, g.W == 0);
+  auto go = [&]<bool UNIFORM>() {
+    if (stream)
+      hipLaunchKernelGGL((paged_decode_kernel<E, HS, M, UNIFORM, true>), grid, dim3(256), 0, st, a, plan, g.W == 0);
+    else
+      hipLaunchKernelGGL((paged_decode_kernel<E, HS, M, UNIFORM, false>), grid, dim3(256), 0, st, a, plan, g.W == 0);
+  };
+  if (plan.ps.d % 16 == 0) go.template operator()<true>();
+  else go.template operator()<false>();
   if (g.W == 0) return;
   const int64_t rows = (int64_t)plan.B * a.nh;
   // four waves a row where a job has eight parts or more on average
   if (g.W >= 8 * g.jobs)
-    hipLaunchKernelGGL((paged_decode_join_kernel<E, HS, 4>), dim3((unsigned)rows), dim3(256), 0, st, a, plan, g.W);
+    hipLaunchKernelGGL((paged_decode_join_kernel<E, HS, M, 4>), dim3((unsigned)rows), dim3(256), 0, st, a, plan, g.W);
   else
-    hipLaunchKernelGGL((paged_decode_join_kernel<E, HS, 1>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, a, plan, g.W);
+    hipLaunchKernelGGL((paged_decode_join_kernel<E, HS, M, 1>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, a, plan, g.W);
 }
 
 template <class E, class P>
@@ -593,13 +637,19 @@ int decode(const P* q, const int64_t* qs, float scale, P* o, float* l, void* ws,
   a.sk = {pa.ks[0], pa.ks[1], pa.ks[2]};
   a.sv = {pa.vs[0], pa.vs[1], pa.vs[2]};
   a.nh = (int)pa.nh; a.nkv = (int)pa.nkv; a.group = (int)(pa.nh / pa.nkv);
-  a.chunks = (a.group + 15) / 16;
+  a.chunks = (int)g.chunks;
   a.scale_log2 = scale * kLog2e;
   a.o = reinterpret_cast<E*>(o); a.l = l; a.ws = static_cast<float*>(ws);
   const hipStream_t st = as_stream(stream);
-  if (pa.hs == 32) launch_decode<E, 32>(a, plan, g, st);
-  else if (pa.hs == 64) launch_decode<E, 64>(a, plan, g, st);
-  else launch_decode<E, 128>(a, plan, g, st);
+  const bool past = g.chunks == 1 &&
+                    pa.num_pages * pa.page_size * pa.nkv * pa.hs * 2 * (int64_t)sizeof(E) >= kStreamBytes;
+  auto go = [&]<int HS>() {
+    if (g.pass == 32) launch_decode<E, HS, 2>(a, plan, g, past, st);
+    else launch_decode<E, HS, 1>(a, plan, g, past, st);
+  };
+  if (pa.hs == 32) go.template operator()<32>();
+  else if (pa.hs == 64) go.template operator()<64>();
+  else go.template operator()<128>();
   return check_launch("paged_attention_decode");
 }
 
@@ -615,7 +665,8 @@ extern "C" int64_t cta_paged_attention_decode_workspace(int64_t B, int64_t nh, i
   if (B <= 0 || nh <= 0 || nkv <= 0 || pages_per_seq <= 0 || page_size <= 0 ||
       (hs != 32 && hs != 64 && hs != 128) || pages_per_seq > ((int64_t)1 << 30) / page_size)
     return 0;
-  return (int64_t)decode_grid(B, nh, nkv, hs, pages_per_seq * page_size, 4).W * 2 * 16 * (hs + 2) * 4;
+  const DecodeGrid g = decode_grid(B, nh, nkv, hs, pages_per_seq * page_size, 4);
+  return (int64_t)g.W * 2 * g.pass * (hs + 2) * 4;
 }
 
 #define CTA_PAGED_DECODE(SUFFIX, TYPE, PTR)                                                       \

@@ -39,7 +39,7 @@ struct PrefillArgs {
   float scale_log2;
   int tiles;  // tiles of 128 rows that a key/value head may have
   int W;      // workgroups that the tiles' cost is dealt to; 0: a workgroup a tile
-  int least;  // ... each of them at least this much
+  int set_up;  // cost of beginning a tile
   E* o;
   float* l;
   float* ws;  // W > 0: O (2 W, 128, HS), then (m, l) (2 W, 128): a workgroup's first and last part
@@ -65,20 +65,20 @@ struct RowTile {
     return at == 0 ? 0 : at == cost ? n : (int)(n * at / cost);
   }
 };
-// Work of a sequence's tiles: tile q costs past + 128 (q + 1), the keys that its last row would see
-// (times group) were the tile full.  Every cost is positive, and the sum of the first q has a
-// closed form.
+// Work of a sequence's tiles: tile q costs base + 128 (q + 1).  That is the keys that its last row
+// would see were the tile full, times group, and as much as kSetUp stages for beginning a tile.
+// Every cost is positive, and the sum of the first q has a closed form.
 struct SeqCost {
   int first, R;
-  int64_t past;
+  int64_t base;
   __device__ __forceinline__ int tiles() const { return (R + BM - 1) / BM; }
-  __device__ __forceinline__ int64_t upto(int64_t q) const { return q * past + BM / 2 * q * (q + 1); }
+  __device__ __forceinline__ int64_t upto(int64_t q) const { return q * base + BM / 2 * q * (q + 1); }
 };
 template <class E>
 __device__ __forceinline__ SeqCost seq_cost(const PrefillArgs<E>& a, const PagedPlan& plan, int b) {
   SeqCost c;
   c.R = tokens_of(plan, a.N, b, c.first) * (int)a.group.d;
-  c.past = (int64_t)plan.keys_to(plan.position(b, c.first) - 1) * a.group.d;
+  c.base = (int64_t)plan.keys_to(plan.position(b, c.first) - 1) * a.group.d + a.set_up;
   return c;
 }
 // Tile x of a head, all sequences' tiles in a row; false: there are fewer (then before is their
@@ -92,7 +92,7 @@ __device__ __forceinline__ bool find_rows(const PrefillArgs<E>& a, const PagedPl
   w.first = uniform(c.first);
   w.R = uniform(c.R);
   w.tile = x - (int)before;
-  w.cost = uniform(c.past) + BM * (int64_t)(w.tile + 1);
+  w.cost = uniform(c.base) + BM * (int64_t)(w.tile + 1);
   w.lo = 0;
   w.hi = w.cost;
   return true;
@@ -118,7 +118,7 @@ __device__ __forceinline__ Deal make_deal(const PrefillArgs<E>& a, const PagedPl
     return c.upto(c.tiles());
   });
   d.units = d.head * a.nkv;
-  d.W = (int)max((int64_t)1, min((int64_t)a.W, d.units / a.least));
+  d.W = (int)max((int64_t)1, min((int64_t)a.W, d.units / (2 * a.set_up)));
   d.slack = d.units / d.W / 8;
   return d;
 }
@@ -136,7 +136,7 @@ __device__ __forceinline__ void find_share(const PrefillArgs<E>& a, const PagedP
   SeqCost c = seq_cost(a, plan, w.b);
   w.first = c.first = uniform(c.first);
   w.R = c.R = uniform(c.R);
-  c.past = uniform(c.past);
+  c.base = uniform(c.base);
   u -= before;
   int q = 0;  // the last tile that begins at or before u
   for (int n = c.tiles(); n > 1;) {
@@ -146,7 +146,7 @@ __device__ __forceinline__ void find_share(const PrefillArgs<E>& a, const PagedP
   }
   u -= c.upto(q);
   w.tile = q;
-  w.cost = c.past + BM * (int64_t)(q + 1);
+  w.cost = c.base + BM * (int64_t)(q + 1);
 }
 // The next tile of the deal (there is one).
 template <class E>
@@ -164,7 +164,7 @@ __device__ __forceinline__ void next_tile(const PrefillArgs<E>& a, const PagedPl
   } while (w.R == 0);
   w.first = uniform(c.first);
   w.tile = 0;
-  w.cost = uniform(c.past) + BM;
+  w.cost = uniform(c.base) + BM;
 }
 // Rows of no sequence count as empty: share i of n of them, for head kvh.
 template <class E, int HS>
@@ -304,6 +304,13 @@ __device__ __forceinline__ float exp2_sum(float* s) {
   return t[0];
 }
 
+// Where a part of a tile keeps the four elements d 32 + 8 g + 4 (lane / 32) .. of row
+// 32 wave + lane % 32.
+template <int HS>
+__device__ __forceinline__ int64_t part_at(int slot, int wave, int d, int g, int lane) {
+  return (int64_t)slot * BM * HS + (((wave * (HS / 32) + d) * 4 + g) * 64 + lane) * 4;
+}
+
 // Writes a lane's part of its row: the result, or the share's part of it (`any`: it had stages).
 template <class E, int HS>
 __device__ __forceinline__ void store_rows(const PrefillArgs<E>& a, const RowTile& w, int slot,
@@ -312,18 +319,18 @@ __device__ __forceinline__ void store_rows(const PrefillArgs<E>& a, const RowTil
   const float l_tot = sum_halves(l_run);
   if (w.tile * BM + in_tile >= w.R) return;
   if (!w.whole()) {
-    const int64_t at = (int64_t)slot * BM + in_tile;
-    float* op = a.ws + at * HS;
+    // in the order of the registers: a wave's store is 1 KiB in a row
     if (any) {
 #pragma unroll
       for (int d = 0; d < HS / 32; ++d)
 #pragma unroll
         for (int g = 0; g < 4; ++g)
-          st4(op + d * 32 + 8 * g + 4 * half, make_float4(oacc[d][4 * g], oacc[d][4 * g + 1],
-                                                          oacc[d][4 * g + 2], oacc[d][4 * g + 3]));
+          st4(a.ws + part_at<HS>(slot, wave_index(), d, g, lane),
+              make_float4(oacc[d][4 * g], oacc[d][4 * g + 1], oacc[d][4 * g + 2], oacc[d][4 * g + 3]));
     }
     if (half == 0)
-      *reinterpret_cast<float2*>(a.ws + (int64_t)2 * a.W * BM * HS + at * 2) = make_float2(mb, l_tot);
+      *reinterpret_cast<float2*>(a.ws + (int64_t)2 * a.W * BM * HS + ((int64_t)slot * BM + in_tile) * 2) =
+          make_float2(mb, l_tot);
     return;
   }
   int token, head;
@@ -762,7 +769,7 @@ __global__ __launch_bounds__(256, HS == 128 ? 1 : 2) void paged_prefill_f32_kern
 }
 
 // Joins the parts of the tiles that several workgroups share, in order, and fills padding rows.  A
-// workgroup has 1024 / HS rows of a tile, a thread four elements of a row.
+// wave has one of the 1 KiB stores that a part consists of, a thread four elements of a row.
 template <class E, int HS>
 __global__ __launch_bounds__(256) void paged_prefill_join_kernel(PrefillArgs<E> a, PagedPlan plan) {
   constexpr int BLOCKS = BM * HS / 1024;  // a tile
@@ -782,16 +789,18 @@ __global__ __launch_bounds__(256) void paged_prefill_join_kernel(PrefillArgs<E> 
   const int64_t edge = deal.edge(w.cost);
   const int w0 = deal.owner(begin + edge), w1 = deal.owner(begin + w.cost - edge - 1);
   if (w0 == w1) return;  // written whole
-  const int r = 1024 / HS * (rest % BLOCKS) + threadIdx.x / (HS / 4), d = 4 * (threadIdx.x % (HS / 4));
+  const int lane = threadIdx.x & 63, store = rest % BLOCKS * 4 + wave_index();
+  const int g4 = store % 4, d32 = store / 4 % (HS / 32), wave = store / (HS / 8);
+  const int r = wave * 32 + lane % 32, d = 32 * d32 + 8 * g4 + 4 * (lane / 32);
   if (w.tile * BM + r >= w.R) return;
   const float2* ml = reinterpret_cast<const float2*>(a.ws + (int64_t)2 * a.W * BM * HS);
-  auto at = [&](int i) { return (int64_t)(2 * i + (i == w0)) * BM + r; };
+  auto slot = [&](int i) { return 2 * i + (i == w0); };
   // four parts' loads in flight at a time
   float m = -INFINITY;
   for (int i = w0; i <= w1; i += 4) {
     float x4[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) x4[j] = ml[at(min(i + j, w1))].x;
+    for (int j = 0; j < 4; ++j) x4[j] = ml[(int64_t)slot(min(i + j, w1)) * BM + r].x;
     m = fmaxf(m, max3_tree(x4));
   }
   const float off = m == -INFINITY ? 0.0f : m;
@@ -802,8 +811,9 @@ __global__ __launch_bounds__(256) void paged_prefill_join_kernel(PrefillArgs<E> 
     float4 v[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      p[j] = ml[at(min(i + j, w1))];
-      v[j] = ld4(a.ws + at(min(i + j, w1)) * HS + d);
+      const int at = slot(min(i + j, w1));
+      p[j] = ml[(int64_t)at * BM + r];
+      v[j] = ld4(a.ws + part_at<HS>(at, wave, d32, g4, lane));
     }
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -827,8 +837,13 @@ __global__ __launch_bounds__(256) void paged_prefill_join_kernel(PrefillArgs<E> 
 
 // Tiles of 128 rows that a key/value head may have (each sequence may end inside one; one more, so
 // that some workgroup is left for padding rows), and the workgroups that their cost is dealt to: as
-// many as the GPU holds at once, two stages or more each.  From four tiles a place on, or where no
-// tile has more than eight stages, a workgroup takes a whole tile (W = 0).
+// many as the GPU holds at once.  With a tile or more for each of these places, or where no tile has
+// more than eight stages, a workgroup takes a whole tile (W = 0): dealing costs a second kernel and
+// more tiles begun.  Measured whole and dealt, us: 4 x 2000 tokens of 16 heads of 64 (two tiles a
+// place) 70 and 99; 8 x 50 to 1500 tokens of 32 over 8 heads of 128 behind up to 2000 (1.1) 108 and
+// 159; 5 x 200 to 2000 FP32 tokens of 12 heads of 64 (0.9) 160 and 112; one of 2000, 32 over 8 heads
+// of 128 (almost one) 58 and 78; 256 tokens behind 60000 cannot be whole tiles: 64 places of 512.
+constexpr int kSetUp = 3;  // stages' time that a tile's lookups, queries and stores take
 struct PrefillGrid {
   int64_t tiles;
   int W, stage;
@@ -841,7 +856,7 @@ PrefillGrid prefill_grid(int64_t B, int64_t N, int64_t nh, int64_t nkv, int64_t 
   const int64_t places = 256 * (elem == 4 ? (hs == 128 ? 1 : 2) : (hs == 32 ? 3 : 2));
   const int64_t about = std::max<int64_t>(1, (N * (nh / nkv) + 64 * std::min(B, N)) / 128) * nkv;
   const int64_t stages = (capacity + g.stage - 1) / g.stage;
-  g.W = about >= 4 * places || stages <= 8 ? 0 : (int)std::min(places, (g.tiles - 1) * nkv * stages / 2);
+  g.W = about >= places || stages <= 8 ? 0 : (int)std::min(places, (g.tiles - 1) * nkv * stages / 2);
   return g;
 }
 
@@ -873,7 +888,7 @@ int prefill(const P* q, const int64_t* qs, int64_t N, float scale, P* o, float* 
   const PrefillGrid g = prefill_grid(pa.B, N, pa.nh, pa.nkv, pa.hs, plan.capacity, sizeof(E));
   const double group = (double)(pa.nh / pa.nkv);
   if (g.tiles * pa.nkv >= (int64_t)1 << 27 ||  // grids, and the work's units in 53 bits
-      (double)g.tiles * pa.nkv * (group * plan.capacity + 128.0 * g.tiles) >= 0x1p53)
+      (double)g.tiles * pa.nkv * (group * (plan.capacity + kSetUp * g.stage) + 128.0 * g.tiles) >= 0x1p53)
     return fail(CTA_ERR_INVALID_ARGUMENT, "size too large");
   if (g.W > 0 && (!ws || !aligned16(ws) ||
                        ws_bytes < cta_paged_attention_prefill_workspace(
@@ -888,7 +903,7 @@ int prefill(const P* q, const int64_t* qs, int64_t N, float scale, P* o, float* 
   a.N = (int)N; a.nh = (int)pa.nh; a.nkv = (int)pa.nkv;
   a.group = FastDiv((uint32_t)(pa.nh / pa.nkv));
   a.scale_log2 = scale * kLog2e;
-  a.tiles = (int)g.tiles; a.W = g.W; a.least = 2 * g.stage * (int)a.group.d;
+  a.tiles = (int)g.tiles; a.W = g.W; a.set_up = kSetUp * g.stage * (int)a.group.d;
   a.o = reinterpret_cast<E*>(o); a.l = l; a.ws = static_cast<float*>(ws);
   const hipStream_t st = as_stream(stream);
   if (pa.hs == 32) launch_prefill<E, 32>(a, plan, st);

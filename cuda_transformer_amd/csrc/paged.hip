@@ -48,7 +48,7 @@ int check_paged_rows(const void* q, const int64_t* qs, int64_t rows, const Paged
                      const void* o, const float* l, int elem, const char* what) {
   if (rows < 0 || rows > (int64_t)1 << 24 || rows * a.nh > (int64_t)1 << 30)
     return fail(CTA_ERR_INVALID_ARGUMENT, "size too large");
-  if (!std::isfinite(scale)) return fail(CTA_ERR_INVALID_ARGUMENT, "scale must be finite");
+  if (!std::isfinite(scale * kLog2e)) return fail(CTA_ERR_INVALID_ARGUMENT, "scale must be finite");
   if (rows * a.nh == 0) return CTA_OK;
   if (!o || !l) return fail(CTA_ERR_INVALID_ARGUMENT, "null output pointer");
   if (!tokens_layout_ok(q, qs, elem) || !aligned16(o))

@@ -177,7 +177,7 @@ int append(const P* q, const int64_t* qs, const P* k, const int64_t* ks, const P
     return fail(CTA_ERR_LAYOUT, "cos and sin must be 16-byte aligned");
   if (N * (pa.nh + 2 * pa.nkv) * pa.hs * (int64_t)sizeof(E) / 32 >= (int64_t)1 << 31)  // threads
     return fail(CTA_ERR_INVALID_ARGUMENT, "size too large");
-  if (N == 0 || pa.B == 0) return CTA_OK;
+  if (N == 0) return CTA_OK;
   if (!tokens_layout_ok(k, ks, sizeof(E)) || !tokens_layout_ok(v, vs, sizeof(E)) ||
       (pa.nh > 0 && (!tokens_layout_ok(q, qs, sizeof(E)) || !q_out || !aligned16(q_out))))
     return fail(CTA_ERR_LAYOUT,

@@ -48,8 +48,8 @@ struct PrefillArgs {
 
 // Tokens of sequence b: first row and count, inside [0, N) whatever cu_q holds.
 __device__ __forceinline__ int tokens_of(const PagedPlan& plan, int N, int b, int& first) {
-  first = max(plan.cu_q[b], 0);
-  return max(min(plan.cu_q[b + 1], N) - first, 0);
+  first = min(max(plan.cu_q[b], 0), N);
+  return max(min(max(plan.cu_q[b + 1], 0), N) - first, 0);
 }
 
 constexpr int BM = 128;              // rows a workgroup
@@ -924,9 +924,16 @@ PrefillGrid prefill_grid(int64_t B, int64_t N, int64_t nh, int64_t nkv, int64_t 
   g.tiles = N * (nh / nkv) / 128 + std::min(B, N) + 1;
   g.stage = elem == 4 ? 32 : 64;
   const int64_t places = 256 * (elem == 4 ? (hs == 128 ? 1 : 2) : (hs == 32 ? 3 : 2));
-  const int64_t about = std::max<int64_t>(1, (N * (nh / nkv) + 64 * std::min(B, N)) / 128) * nkv;
+  const int64_t group = nh / nkv;
+  const int64_t about = std::max<int64_t>(1, (N * group + 64 * std::min(B, N)) / 128) * nkv;
   const int64_t stages = (capacity + g.stage - 1) / g.stage;
-  g.W = about >= places || stages <= 8 ? 0 : (int)std::min(places, (g.tiles - 1) * nkv * stages / 2);
+  // Units of work, whatever cu_q holds: a deal needs them in 53 bits, and a tile's times its stages
+  // in 63.
+  const double most = (double)N * group / 128 + 1;
+  const double units = (double)B * most * nkv * ((double)group * (capacity + kSetUp * g.stage) + 128 * most);
+  g.W = about >= places || stages <= 8 || units >= 0x1p53 || units * stages >= 0x1p62 * (B * most * nkv)
+            ? 0
+            : (int)std::min(places, (g.tiles - 1) * nkv * stages / 2);
   return g;
 }
 
@@ -958,10 +965,7 @@ int prefill(const P* q, const int64_t* qs, int64_t N, float scale, P* o, float* 
     return rc;
   if (N * pa.nh == 0) return CTA_OK;
   const PrefillGrid g = prefill_grid(pa.B, N, pa.nh, pa.nkv, pa.hs, plan.capacity, sizeof(E));
-  const double group = (double)(pa.nh / pa.nkv);
-  if (g.tiles * pa.nkv >= (int64_t)1 << 27 ||  // grids, and the work's units in 53 bits
-      (double)g.tiles * pa.nkv * (group * (plan.capacity + kSetUp * g.stage) + 128.0 * g.tiles) >= 0x1p53)
-    return fail(CTA_ERR_INVALID_ARGUMENT, "size too large");
+  if (g.tiles * pa.nkv >= (int64_t)1 << 31) return fail(CTA_ERR_INVALID_ARGUMENT, "size too large");
   if (g.W > 0 && (!ws || !aligned16(ws) ||
                        ws_bytes < cta_paged_attention_prefill_workspace(
                                       pa.B, N, pa.nh, pa.nkv, pa.hs, pa.pages_per_seq, pa.page_size)))

@@ -155,8 +155,11 @@ def test_decode_long_and_ragged(cuda, dtype, ps):
 
 
 @pytest.mark.parametrize("dtype", ALL)
-def test_decode_many_sequences(cuda, dtype):
-    lens = [(37 * i) % 61 for i in range(300)]
+@pytest.mark.parametrize("longest", [61, 2300])
+def test_decode_many_sequences(cuda, dtype, longest):
+    """More sequences than a wave's lanes, short ones only and with long ones among them."""
+    lens = [(37 * i) % 61 for i in range(150)]
+    lens[7], lens[140] = longest, longest // 2
     check_decode(decode_inputs(dtype, 2, 1, 32, 16, lens, seed=4), cuda)
 
 
@@ -280,9 +283,52 @@ def test_prefill_few_rows_long_cache(cuda, dtype, ps):
 
 
 @pytest.mark.parametrize("dtype", ALL)
-def test_prefill_many_sequences(cuda, dtype):
-    lens = [(29 * i) % 41 for i in range(150)]
-    check_prefill(make(DTYPES[dtype], 2, 1, 32, 16, lens, [n // 3 for n in lens], seed=22), cuda)
+@pytest.mark.parametrize("longest", [41, 1500])
+def test_prefill_many_sequences(cuda, dtype, longest):
+    lens = [(29 * i) % 41 for i in range(100)]
+    news = [n // 3 for n in lens]
+    lens[70], lens[99] = longest, longest // 2
+    check_prefill(make(DTYPES[dtype], 2, 1, 32, 16, lens, news, seed=22), cuda)
+
+
+@pytest.mark.parametrize("dtype", ALL)
+@pytest.mark.parametrize("hs,ps", [(32, 16), (64, 40), (128, 64)])
+def test_prefill_uneven_tiles(cuda, dtype, hs, ps):
+    """Tiles of very different cost, cut anywhere and joined, beside rows of padding, an unmapped page
+    and sequences without new tokens."""
+    d = make(DTYPES[dtype], 6, 2, hs, ps, [1300, 40, 900, 0, 700, 300], [60, 40, 130, 0, 0, 1], seed=29,
+             holes=[(0, 1)])
+    d["q"] = torch.cat([d["q"], torch.full((40, 6, hs), torch.nan, dtype=d["q"].dtype)])
+    check_prefill(d, cuda)
+
+
+def test_prefill_fp32_of_any_magnitude_in_parts(cuda):
+    """Values beyond the split's range in the middle of a long cache: the parts of the tile that see
+    them agree with those that do not."""
+    d = make(torch.float32, 4, 2, 64, 16, [1500], [20], seed=30)
+    d["v_cache"][d["table"][0, 40]] *= 2.0 ** 110
+    d["k_cache"][d["table"][0, 80]] *= 2.0 ** -100
+    check_prefill(d, cuda)
+
+
+def test_plans_of_any_values(cuda):
+    """Lengths, pages and row counts that make no sense give some result and touch nothing else."""
+    g = torch.Generator().manual_seed(61)
+    for dtype in ("float32", "bfloat16"):
+        d = to(make(DTYPES[dtype], 4, 2, 64, 16, [700, 40, 900, 33], [40, 40, 20, 3], seed=31, garbage=0.0), cuda)
+        guard = torch.full((1 << 20,), 3.0, device=cuda)
+        for _ in range(4):
+            for name in ("table", "lens", "cu"):
+                x = torch.randint(-(2 ** 31), 2 ** 31 - 1, d[name].shape, generator=g, dtype=torch.int64)
+                small = torch.randint(-60, 200, d[name].shape, generator=g)
+                pick = torch.rand(d[name].shape, generator=g) < 0.5
+                d[name].copy_(torch.where(pick, x, small).to(torch.int32))
+            c = (d["k_cache"], d["v_cache"], d["table"], d["lens"])
+            ops.paged_kv_append(d["k"], d["v"], *c, d["cu"])
+            ops.paged_attention_decode(d["q"][:4], *c)
+            ops.paged_attention_prefill(d["q"], *c, d["cu"])
+            torch.cuda.synchronize()
+        assert (guard == 3.0).all()
 
 
 @pytest.mark.parametrize("dtype", ALL)
@@ -380,6 +426,10 @@ def test_empty_calls(cuda):
         O, L = ops.paged_attention_prefill(torch.ones(3, 4, 64, dtype=dt, device=cuda), *c[:2], none,
                                            d["lens"][:0], d["cu"][:1])
         assert (O == 0).all() and torch.isneginf(L).all()
+        q = torch.randn(3, 4, 64, device=cuda).to(dt)
+        cos = torch.rand(48, 32, device=cuda)
+        x = torch.ones(3, 2, 64, dtype=dt, device=cuda)
+        assert torch.equal(ops.paged_kv_append(x, x, *c[:2], none, d["lens"][:0], d["cu"][:1], q, cos, cos), q)
         no_pages = torch.empty(2, 0, dtype=torch.int32, device=cuda)
         O, L = ops.paged_attention_decode(torch.ones(2, 4, 64, dtype=dt, device=cuda), *c[:2], no_pages, d["lens"] + 5)
         assert (O == 0).all() and torch.isneginf(L).all()

@@ -292,6 +292,17 @@ __device__ __forceinline__ void exponents(float (&s)[N], float c, float& mb, M&&
     mb = mb_new;
   }
 }
+// Exponents of a 32-key tile (register r: key R(r, half)) that do not count -> -inf: bit j of `ok` says
+// whether key j holds one, of which the row sees the first `seen`.  Two instructions a value.
+__device__ __forceinline__ void mask_tile(float* s, uint32_t ok, int seen, int half) {
+  ok = seen >= 32 ? ok : seen <= 0 ? 0 : ok & ((1u << seen) - 1);
+  ok >>= 4 * half;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) {
+    const uint32_t keep = (uint32_t)__builtin_amdgcn_sbfe((int)ok, mfma_row(r, 0), 1);  // 0 or all ones
+    s[r] = __uint_as_float((keep & __float_as_uint(s[r])) | (~keep & 0xff800000u));
+  }
+}
 // 2^s in place, and their sum.
 template <int N>
 __device__ __forceinline__ float exp2_sum(float* s) {
@@ -372,8 +383,12 @@ __device__ __forceinline__ s16x4 ld_transposed(const void* p) {
 }
 
 // UNIFORM: a group of 16 keys lies in one page (the page size is a multiple of 16).
+// Three waves a SIMD at hs 32, two else: registers would allow more, but fewer workgroups walk the
+// same keys closer together (4 x 2000 tokens of 16 heads: hs 32 50.6 us with three and 59.8 with
+// four, hs 64 65.5 with two and 66.2 with three).
 template <class E, int HS, bool DEAL, bool UNIFORM>
-__global__ __launch_bounds__(256, HS == 32 ? 3 : 2) void paged_prefill_half_kernel(PrefillArgs<E> a, PagedPlan plan) {
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HS == 32 ? 3 : 2, HS == 32 ? 3 : 2)))
+void paged_prefill_half_kernel(PrefillArgs<E> a, PagedPlan plan) {
   constexpr int BN = 64;           // keys a stage, one step of the softmax
   constexpr int RB = 2 * HS;       // bytes of a row
   constexpr int STAGE = BN * RB;   // bytes of K (or V) a stage
@@ -416,19 +431,20 @@ __global__ __launch_bounds__(256, HS == 32 ? 3 : 2) void paged_prefill_half_kern
   const E* kb = a.k + w.kvh * a.sk.h;
   const E* vb = a.v + w.kvh * a.sv.h;
 
-  // Any page size.  Page of key `lane` of a stage, by waves 0 (K) and 1 (V); -1: none.
+  // Any page size.  Page of key `lane` of a stage, by waves 2 (K) and 3 (V), which idle where a tile
+  // has few rows; -1: none.
   auto look_up = [&](int stage) {
     const int j = stage * BN + lane;
-    return wave < 2 && stage < s_end && j < v.n_keys ? table[plan.ps.div(j)] : -1;
+    return wave >= 2 && stage < s_end && j < v.n_keys ? table[plan.ps.div(j)] : -1;
   };
   auto put = [&](int stage, int page) {
-    if (wave >= 2) return;
+    if (wave < 2) return;
     const int j = stage * BN + lane, row = j - plan.ps.div(j) * (int)plan.ps.d;
     const bool ok = (uint32_t)page < (uint32_t)plan.num_pages;
-    const E* p = wave == 0 ? kb + page * a.sk.a + row * a.sk.r : vb + page * a.sv.a + row * a.sv.r;
-    row_at[stage & 1][wave][lane] = ok ? (uint64_t)p : (uint64_t)kZeroRow;
+    const E* p = wave == 2 ? kb + page * a.sk.a + row * a.sk.r : vb + page * a.sv.a + row * a.sv.r;
+    row_at[stage & 1][wave - 2][lane] = ok ? (uint64_t)p : (uint64_t)kZeroRow;
     const uint64_t all = __ballot(ok);
-    if (tid == 0) holds[stage & 3] = all;
+    if (tid == 128) holds[stage & 3] = all;
   };
   // UNIFORM.  Where 64 groups of 16 keys begin in the pools, a group a lane, from stage tp on
   // (`mapped`: those with a page), and the pages of the next 64.
@@ -542,11 +558,8 @@ __global__ __launch_bounds__(256, HS == 32 ? 3 : 2) void paged_prefill_half_kern
         s, a.scale_log2, mb,
         [&] {
           if (j0 + BN <= v.lo && ~ok == 0) return;
-#pragma unroll
-          for (int r = 0; r < 32; ++r) {
-            const int j = 32 * (r >> 4) + mfma_row(r & 15, half);
-            if (j0 + j >= v.keys || !(ok >> j & 1)) s[r] = -INFINITY;
-          }
+          mask_tile(s, (uint32_t)ok, v.keys - j0, half);
+          mask_tile(s + 16, (uint32_t)(ok >> 32), v.keys - j0 - 32, half);
         },
         [&](float alpha) {
           l_run *= alpha;
@@ -648,30 +661,27 @@ __global__ __launch_bounds__(256, HS == 128 ? 1 : 2) void paged_prefill_f32_kern
   for (int d = 0; d < HS / 32; ++d) { oacc[d] = zero16(); olow[d] = zero16(); }
   float mb = -INFINITY, l_run = 0.0f;
 
-  // Page of a stage's key lane % 32, in wave 0: lanes 0 .. 31 for K, 32 .. 63 for V.
+  // Page of a stage's key lane % 32, in wave 3, which idles where a tile has few rows: lanes 0 .. 31
+  // for K, 32 .. 63 for V.
   const int32_t* table = plan.table + w.b * plan.table_stride;
   auto look_up = [&](int stage) {
     const int j = stage * BN + col;
-    return wave == 0 && stage < s_end && j < v.n_keys ? table[plan.ps.div(j)] : -1;
+    return wave == 3 && stage < s_end && j < v.n_keys ? table[plan.ps.div(j)] : -1;
   };
   const float* kb = a.k + w.kvh * a.sk.h;
   const float* vb = a.v + w.kvh * a.sv.h;
   auto put = [&](int stage, int page) {
-    if (wave != 0) return;
+    if (wave != 3) return;
     const int j = stage * BN + col, row = j - plan.ps.div(j) * (int)plan.ps.d;
     const bool ok = (uint32_t)page < (uint32_t)plan.num_pages;
     const float* p = half == 0 ? kb + page * a.sk.a + row * a.sk.r : vb + page * a.sv.a + row * a.sv.r;
     row_at[stage & 1][half][col] = ok ? (uint64_t)p : (uint64_t)kZeroRow;
     const uint64_t all = __ballot(ok);
-    if (tid == 0) holds[stage & 3] = (uint32_t)all;
+    if (tid == 192) holds[stage & 3] = (uint32_t)all;
   };
   auto mask = [&](float (&s)[16], int j0, uint32_t ok) {
     if (j0 + BN <= v.lo && ~ok == 0) return;
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      const int j = mfma_row(r, half);
-      if (j0 + j >= v.keys || !(ok >> j & 1)) s[r] = -INFINITY;
-    }
+    mask_tile(s, ok, v.keys - j0, half);
   };
 
   // K unit (d8, key), d 8 d8 .. of a key, lies at d8 * 32 + (key ^ (d8 & 7)); V unit (d, sh), the

@@ -848,11 +848,16 @@ __global__ __launch_bounds__(256, HS == 128 ? 1 : 2) void paged_prefill_f32_kern
   });
 }
 
-// Joins the parts of the tiles that several workgroups share, in order, and fills padding rows.  A
-// wave has one of the 1 KiB stores that a part consists of, a thread four elements of a row.
-template <class E, int HS>
+// Joins the parts of the tiles that several workgroups share, in order, and fills padding rows.  A part
+// consists of 1 KiB stores; a wave has SETS of them that share their rows, a thread four elements of a
+// row from each, and the loads of FLIGHT parts at a time in flight.  Few parts a tile: SETS = 4, as the
+// deal costs a wave more than its loads (a prompt of 2000 tokens, 32 over 8 heads of 128: 77 us with
+// one, 66 with four).  Many: SETS = 1 and more waves walk them (two drafts of 4 tokens behind 60000:
+// 109 us with four, 103 with one).
+template <class E, int HS, int SETS>
 __global__ __launch_bounds__(256) void paged_prefill_join_kernel(PrefillArgs<E> a, PagedPlan plan) {
-  constexpr int BLOCKS = BM * HS / 1024;  // a tile
+  constexpr int BLOCKS = BM * HS / (1024 * SETS);  // a tile
+  constexpr int FLIGHT = SETS == 4 ? 2 : 4;
   const int x = blockIdx.x / (BLOCKS * a.nkv), rest = blockIdx.x - x * BLOCKS * a.nkv;
   RowTile w;
   w.kvh = rest / BLOCKS;
@@ -869,13 +874,12 @@ __global__ __launch_bounds__(256) void paged_prefill_join_kernel(PrefillArgs<E> 
   const int64_t edge = deal.edge(w.cost);
   const int w0 = deal.owner(begin + edge), w1 = deal.owner(begin + w.cost - edge - 1);
   if (w0 == w1) return;  // written whole
-  const int lane = threadIdx.x & 63, store = rest % BLOCKS * 4 + wave_index();
-  const int g4 = store % 4, d32 = store / 4 % (HS / 32), wave = store / (HS / 8);
-  const int r = wave * 32 + lane % 32, d = 32 * d32 + 8 * g4 + 4 * (lane / 32);
+  const int lane = threadIdx.x & 63, set = rest % BLOCKS * 4 + wave_index();
+  const int g0 = set * SETS % 4, d32 = set * SETS / 4 % (HS / 32), wave = set * SETS / (HS / 8);
+  const int r = wave * 32 + lane % 32;
   if (w.tile * BM + r >= w.R) return;
   const float2* ml = reinterpret_cast<const float2*>(a.ws + (int64_t)2 * a.W * BM * HS);
   auto slot = [&](int i) { return 2 * i + (i == w0); };
-  // four parts' loads in flight at a time
   float m = -INFINITY;
   for (int i = w0; i <= w1; i += 4) {
     float x4[4];
@@ -885,34 +889,44 @@ __global__ __launch_bounds__(256) void paged_prefill_join_kernel(PrefillArgs<E> 
   }
   const float off = m == -INFINITY ? 0.0f : m;
   float l = 0.0f;
-  float4 o = zero4();
-  for (int i = w0; i <= w1; i += 4) {
-    float2 p[4];
-    float4 v[4];
+  float4 o[SETS];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+  for (int g = 0; g < SETS; ++g) o[g] = zero4();
+  for (int i = w0; i <= w1; i += FLIGHT) {
+    float2 p[FLIGHT];
+    float4 v[FLIGHT][SETS];
+#pragma unroll
+    for (int j = 0; j < FLIGHT; ++j) {
       const int at = slot(min(i + j, w1));
       p[j] = ml[(int64_t)at * BM + r];
-      v[j] = ld4(a.ws + part_at<HS>(at, wave, d32, g4, lane));
+#pragma unroll
+      for (int g = 0; g < SETS; ++g) v[j][g] = ld4(a.ws + part_at<HS>(at, wave, d32, g0 + g, lane));
     }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int j = 0; j < FLIGHT; ++j) {
       // a share without stages has written no O
       if (i + j > w1 || (p[j].x == -INFINITY && p[j].y == 0.0f)) continue;
       const float f = fast_exp2(p[j].x - off);
       l = fmaf(f, p[j].y, l);
-      o.x = fmaf(f, v[j].x, o.x); o.y = fmaf(f, v[j].y, o.y);
-      o.z = fmaf(f, v[j].z, o.z); o.w = fmaf(f, v[j].w, o.w);
+#pragma unroll
+      for (int g = 0; g < SETS; ++g) {
+        const float4 x = v[j][g];
+        o[g].x = fmaf(f, x.x, o[g].x); o[g].y = fmaf(f, x.y, o[g].y);
+        o[g].z = fmaf(f, x.z, o[g].z); o[g].w = fmaf(f, x.w, o[g].w);
+      }
     }
   }
   int token, head;
   row_of(a, w, w.tile * BM + r, token, head);
   const int64_t to = (int64_t)token * a.nh + head;
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-  E* op = a.o + to * HS + d;
-  op[0] = (E)(o.x * inv); op[1] = (E)(o.y * inv);
-  op[2] = (E)(o.z * inv); op[3] = (E)(o.w * inv);
-  if (d == 0) a.l[to] = l == 0.0f ? -INFINITY : m * kLn2 + logf(l);
+#pragma unroll
+  for (int g = 0; g < SETS; ++g) {
+    E* op = a.o + to * HS + 32 * d32 + 8 * (g0 + g) + 4 * (lane / 32);
+    op[0] = (E)(o[g].x * inv); op[1] = (E)(o[g].y * inv);
+    op[2] = (E)(o[g].z * inv); op[3] = (E)(o[g].w * inv);
+  }
+  if (g0 == 0 && d32 == 0 && lane < 32) a.l[to] = l == 0.0f ? -INFINITY : m * kLn2 + logf(l);
 }
 
 // Tiles of 128 rows that a key/value head may have (each sequence may end inside one; one more, so
@@ -960,9 +974,14 @@ void launch_prefill(const PrefillArgs<E>& a, const PagedPlan& plan, hipStream_t 
   };
   if (a.W > 0) go.template operator()<true>();
   else go.template operator()<false>();
-  if (a.W > 0)
-    hipLaunchKernelGGL((paged_prefill_join_kernel<E, HS>), dim3((unsigned)((int64_t)a.tiles * a.nkv * (BM * HS / 1024))),
-                       dim3(256), 0, st, a, plan);
+  if (a.W == 0) return;
+  auto join = [&]<int SETS>() {
+    const int64_t blocks = (int64_t)a.tiles * a.nkv * (BM * HS / (1024 * SETS));
+    hipLaunchKernelGGL((paged_prefill_join_kernel<E, HS, SETS>), dim3((unsigned)blocks), dim3(256), 0, st, a, plan);
+  };
+  // more than eight workgroups a tile, at least: many parts
+  if (a.W > 8 * (int64_t)a.tiles * a.nkv) join.template operator()<1>();
+  else join.template operator()<4>();
 }
 
 template <class E, class P>

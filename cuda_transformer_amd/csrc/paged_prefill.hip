@@ -931,12 +931,17 @@ __global__ __launch_bounds__(256) void paged_prefill_join_kernel(PrefillArgs<E> 
 
 // Tiles of 128 rows that a key/value head may have (each sequence may end inside one; one more, so
 // that some workgroup is left for padding rows), and the workgroups that their cost is dealt to: as
-// many as the GPU holds at once.  With a tile or more for each of these places, or where no tile has
-// more than eight stages, a workgroup takes a whole tile (W = 0): dealing costs a second kernel and
-// more tiles begun.  Measured whole and dealt, us: 4 x 2000 tokens of 16 heads of 64 (two tiles a
-// place) 70 and 99; 8 x 50 to 1500 tokens of 32 over 8 heads of 128 behind up to 2000 (1.1) 108 and
-// 159; 5 x 200 to 2000 FP32 tokens of 12 heads of 64 (0.9) 160 and 112; one of 2000, 32 over 8 heads
-// of 128 (almost one) 58 and 78; 256 tokens behind 60000 cannot be whole tiles: 64 places of 512.
+// many as the GPU holds at once.  Dealing costs a second kernel, parts written and read, and more
+// tiles begun, so a workgroup takes a whole tile (W = 0) where
+//  * there is a tile or more for each of these places.  Whole and dealt, us: 4 x 2000 tokens of 16
+//    heads of 64 in BF16 (two tiles a place) 70 and 99; 8 x 50 to 1500 of 32 over 8 heads of 128 behind
+//    up to 2000 (1.1) 108 and 159; but 5 x 200 to 2000 FP32 tokens of 12 heads of 64 (0.9) 155 and 104;
+//  * or the longest tile, by the table's width, has few stages: 8 in FP32; in the 16-bit types 14, and
+//    up to 20 more as the places fill.  One BF16 sequence of 32 over 8 heads of 128: 700 tokens (11
+//    stages, 0.34) 22 and 34, 2000 (32, 0.98) 55 and 66, 128 behind 900 (17, 0.06) 28.9 and 28.2, 1000
+//    behind 4000 (79, 0.48) 110 and 105, 500 behind 4000 (71, 0.25) 99 and 61; 16 x up to 150 behind
+//    up to 2000 (34, 0.7) 52 and 36.  FP32: 2 x 128 behind 300 (14, 0.1) 33 and 30.
+// 256 tokens behind 60000 cannot be whole tiles: 64 places of 512.
 constexpr int kSetUp = 3;  // stages' time that a tile's lookups, queries and stores take
 struct PrefillGrid {
   int64_t tiles;
@@ -955,7 +960,8 @@ PrefillGrid prefill_grid(int64_t B, int64_t N, int64_t nh, int64_t nkv, int64_t 
   // in 63.
   const double most = (double)N * group / 128 + 1;
   const double units = (double)B * most * nkv * ((double)group * (capacity + kSetUp * g.stage) + 128 * most);
-  g.W = about >= places || stages <= 8 || units >= 0x1p53 || units * stages >= 0x1p62 * (B * most * nkv)
+  const int64_t few = elem == 4 ? 8 : 14 + 20 * about / places;
+  g.W = about >= places || stages <= few || units >= 0x1p53 || units * stages >= 0x1p62 * (B * most * nkv)
             ? 0
             : (int)std::min(places, (g.tiles - 1) * nkv * stages / 2);
   return g;

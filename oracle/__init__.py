@@ -20,9 +20,11 @@ Pinning (tests/test_oracle.py, all CPU):
   * softmax — row sums, shift invariance, torch autograd, finite differences.
   * layernorm — torch.nn.functional.layer_norm + autograd, normalisation invariants.
   * naive attention — torch math of test/test_causal_self_attn.py:10-30 + autograd.
+  * paged (appends to and attention over a paged key/value cache; no reference kernel) — float64
+    formulas token by token, pinned in tests/test_paged_cpu.py.
 Mutation tests plant plausible mistakes (wrong scale, dropped mask, transposed operand, missing
 delta term, a dropped or mis-differentiated tanh-GELU term) in copies of the oracle and check that these checks catch them.
 """
-from . import attention, elementwise, linear  # noqa: F401
+from . import attention, elementwise, linear, paged  # noqa: F401
 
-__all__ = ["attention", "elementwise", "linear"]
+__all__ = ["attention", "elementwise", "linear", "paged"]

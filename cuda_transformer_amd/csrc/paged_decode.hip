@@ -575,8 +575,11 @@ __global__ __launch_bounds__(256) void paged_decode_join_kernel(DecodeArgs<E> a,
 }
 
 // How a call is laid out.  pass: query heads that a pass over K and V serves (16 M).  W: workgroups
-// that the tiles are dealt to, two a CU, or 0 where every job is one workgroup's (direct): up to four
-// tiles a job are walked in the time that the second kernel takes.
+// that the tiles are dealt to, two a CU, or 0 where every job is one workgroup's (direct): up to five
+// tiles a job are walked in the time that the deal and the second kernel take, and up to eight where
+// the jobs alone fill the GPU.  Dealt and direct, us, BF16, 32 over 8 heads of 128 (128 keys a tile): 8
+// sequences of 600 (5 tiles) 12.5 and 11.3, 4 of 750 (6) 10.7 and 12.6; 64 of 1000 (8) 46.1 and 43.6, of
+// 50 to 1000 25.0 and 23.5, of 50 to 2000 (16) 36.2 and 39.4.
 struct DecodeGrid {
   int64_t chunks, jobs;
   int pass, W;
@@ -588,7 +591,8 @@ DecodeGrid decode_grid(int64_t B, int64_t nh, int64_t nkv, int64_t hs, int64_t c
   g.chunks = (nh / nkv + g.pass - 1) / g.pass;
   g.jobs = B * nkv * g.chunks;
   const int64_t tiles = (capacity + tile_keys(hs, elem) - 1) / tile_keys(hs, elem);
-  g.W = tiles <= 4 ? 0 : (int)std::min<int64_t>(g.jobs * tiles, 512);
+  const int64_t places = 512;
+  g.W = tiles <= (g.jobs < places ? 5 : 8) ? 0 : (int)std::min<int64_t>(g.jobs * tiles, places);
   return g;
 }
 

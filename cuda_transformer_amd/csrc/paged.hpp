@@ -88,7 +88,7 @@ __device__ __forceinline__ int64_t dpp(int64_t v) {
 }
 // Sums of the lanes' values up to and with each lane, all 64 active: shifts by 1, 2, 4 and 8 inside rows
 // of 16, then the last lane of row 0 into row 1 and of row 2 into row 3, and lane 31 into the upper rows.
-// (33 FP32 sequences of up to 4000 tokens, decode: 13.3 us with shuffles, 12.5 so; a prompt of 128 tokens
+// (33 FP32 sequences of up to 4000 tokens, decode: 13.3 us with shuffles, 12.8 so; a prompt of 128 tokens
 // behind 900: 28.1 and 26.9.)
 template <class T>
 __device__ __forceinline__ T wave_scan(T v) {

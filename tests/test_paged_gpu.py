@@ -164,6 +164,16 @@ def test_decode_many_sequences(cuda, dtype, longest):
 
 
 @pytest.mark.parametrize("dtype", ALL)
+@pytest.mark.parametrize("ps", [16, 20])
+def test_decode_a_workgroup_each(cuda, dtype, ps):
+    """As many jobs as the GPU holds workgroups, up to eight tiles each, some empty."""
+    longest = 500 if dtype == "float32" else 1000
+    lens = [(29 * i) % 41 for i in range(128)]
+    lens[3], lens[70], lens[127] = longest, longest // 2 + 1, longest - 129
+    check_decode(decode_inputs(dtype, 8, 4, 128, ps, lens, seed=5), cuda)
+
+
+@pytest.mark.parametrize("dtype", ALL)
 @pytest.mark.parametrize("ps", [16, 10, 128])
 def test_decode_unmapped_pages(cuda, dtype, ps):
     """Holes in the table, whole sequences without a page, bad page numbers, lengths beyond the pages
@@ -299,6 +309,15 @@ def test_prefill_uneven_tiles(cuda, dtype, hs, ps):
     d = make(DTYPES[dtype], 6, 2, hs, ps, [1300, 40, 900, 0, 700, 300], [60, 40, 130, 0, 0, 1], seed=29,
              holes=[(0, 1)])
     d["q"] = torch.cat([d["q"], torch.full((40, 6, hs), torch.nan, dtype=d["q"].dtype)])
+    check_prefill(d, cuda)
+
+
+@pytest.mark.parametrize("dtype", ALL)
+@pytest.mark.parametrize("hs,ps", [(32, 24), (64, 16), (128, 64)])
+def test_prefill_tiles_of_few_parts(cuda, dtype, hs, ps):
+    """Whole prompts and continued ones whose tiles two or three workgroups share."""
+    lens, news = ([490, 300], [390, 300]) if dtype == "float32" else ([1000, 930], [600, 450])
+    d = make(DTYPES[dtype], 4, 2, hs, ps, lens, news, seed=33, holes=[(1, 2)])
     check_prefill(d, cuda)
 
 

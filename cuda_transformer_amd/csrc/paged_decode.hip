@@ -28,7 +28,7 @@
 //  * FP32 runs on the FP32 MFMA (16x16x4).
 // Measured: 64 sequences of 500 to 8000 tokens, 32 over 8 heads of 128 in BF16 (743 MB) 124 us, 6.1 TB/s
 // (a plain copy reaches 5.8); two of 60000 and 130000, 32 over 4 in FP16 (424 MB) 71 us and 5 for the
-// join; 33 FP32 sequences of up to 4000, 12 over 4 heads of 32 (19 MB) 12.8 us and 8 of up to 251, 6
+// join; 33 FP32 sequences of up to 4000, 12 over 4 heads of 32 (19 MB) 12.5 us and 8 of up to 251, 6
 // heads of 64, 7.3 us: chains of dependent steps.
 #include "paged.hpp"
 
